@@ -4,7 +4,8 @@ A from-scratch sm_100a implementation of the four operators of
 baodii/flash_attention_factory (loop / reduce x fp16 / FP8 KV cache) behind a
 C ABI (``include/paged_attention_b200.h``).  ``flash_attention_factory_b200.lib``
 mirrors the reference's ``lib`` package: four modules, each with ``run(...)``
-taking the reference's positional arguments.
+taking the reference's positional arguments, and beside them the operators that the reference
+lacks (attention over an int8 cache).
 
 There is no CPU fallback: every operator raises if the CUDA library is missing
 or no CUDA device is present.
@@ -13,6 +14,7 @@ from ._cabi import (  # noqa: F401
     KV_F16,
     KV_FP8_E4M3,
     KV_FP8_E5M2,
+    KV_INT8,
     PaParams,
     PaPolicyInfo,
     device_status,

@@ -12,6 +12,7 @@ from pathlib import Path
 KV_F16 = 0
 KV_FP8_E5M2 = 1
 KV_FP8_E4M3 = 2
+KV_INT8 = 3
 
 PA_OK = 0
 PA_ERR_UNSUPPORTED = 1
@@ -29,6 +30,8 @@ EXPORTED_SYMBOLS = (
     "launch_kernels_reduce",
     "launch_kernels_fp8_loop",
     "launch_kernels_fp8_reduce",
+    "launch_kernels_int8_loop",
+    "launch_kernels_int8_reduce",
     "launch_kernels_reduce_static_scratch",
     "pa_reshape_and_cache",
     "pa_query_policy",
@@ -186,7 +189,7 @@ MULTI_GPU_HOST_ONLY = 1
 GATHER_BY_SEQUENCE, GATHER_BY_KV_HEAD = 0, 1
 
 ENTRY_IDS = {"launch_kernels_loop": 0, "launch_kernels_reduce": 1, "launch_kernels_fp8_loop": 2,
-             "launch_kernels_fp8_reduce": 3}
+             "launch_kernels_fp8_reduce": 3, "launch_kernels_int8_loop": 4, "launch_kernels_int8_reduce": 5}
 
 
 def library_path() -> Path:
@@ -214,7 +217,7 @@ def load_library() -> ctypes.CDLL:
     lib = ctypes.CDLL(str(path))
     launcher_args = [ctypes.POINTER(PaParams), ctypes.c_void_p, ctypes.POINTER(ctypes.c_float)]
     for name in ("launch_kernels_loop", "launch_kernels_reduce", "launch_kernels_fp8_loop",
-                 "launch_kernels_fp8_reduce"):
+                 "launch_kernels_fp8_reduce", "launch_kernels_int8_loop", "launch_kernels_int8_reduce"):
         fn = getattr(lib, name)
         fn.argtypes = launcher_args
         fn.restype = ctypes.c_int

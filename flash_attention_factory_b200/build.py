@@ -33,6 +33,8 @@ SOURCES = [
     "launch_kernels_reduce.cu",
     "launch_kernels_fp8_loop.cu",
     "launch_kernels_fp8_reduce.cu",
+    "launch_kernels_int8_loop.cu",
+    "launch_kernels_int8_reduce.cu",
     "cache_write.cu",
 ]
 # the aid library links its own copy of the shared host pieces and nothing of the product

@@ -21,6 +21,8 @@ def _kv_dtype(cache: torch.Tensor) -> int:
         return _cabi.KV_FP8_E4M3
     if cache.dtype in (torch.float8_e5m2, torch.uint8):
         return _cabi.KV_FP8_E5M2
+    if cache.dtype == torch.int8:
+        return _cabi.KV_INT8
     raise RuntimeError(f"unsupported cache dtype {cache.dtype}")
 
 
@@ -30,8 +32,8 @@ def reshape_and_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.T
                       k_scale_per_block=None, v_scale_per_block=None) -> None:
     """key/value fp16 [T, HK, D] -> caches at slot_mapping[t] = block_id * block_size + row.
 
-    Negative slots are skipped.  FP8 caches store round-to-nearest-even(x / scale),
-    saturating, where scale is `fp8_scale` or, when given, the entry of the token's KV head
+    Negative slots are skipped.  FP8 and int8 caches store round-to-nearest-even(x / scale),
+    saturating (int8: to -127 .. 127), where scale is `fp8_scale` or, when given, the entry of the token's KV head
     in `k_scale_per_head` / `v_scale_per_head` (float32 [HK]) or of its block and KV head in
     `k_scale_per_block` / `v_scale_per_block` (float32 [num_blocks, HK]); the attention
     operators take the same scale arguments.  Asynchronous on torch's current stream.

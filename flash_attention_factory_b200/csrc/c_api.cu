@@ -8,6 +8,8 @@ int read_status_loop(int *v);
 int read_status_reduce(int *v);
 int read_status_fp8_loop(int *v);
 int read_status_fp8_reduce(int *v);
+int read_status_int8_loop(int *v);
+int read_status_int8_reduce(int *v);
 
 } // namespace pa
 
@@ -53,8 +55,8 @@ PA_API int pa_query_policy(uint32_t head_size, uint32_t block_size, uint32_t gro
 PA_API int pa_device_status(void) {
   cudaError_t err = cudaDeviceSynchronize();
   if (err != cudaSuccess) return pa::fail(PA_ERR_CUDA, "cudaDeviceSynchronize failed: %s", cudaGetErrorString(err));
-  int (*readers[4])(int *) = {pa::read_status_loop, pa::read_status_reduce, pa::read_status_fp8_loop,
-                              pa::read_status_fp8_reduce};
+  int (*readers[])(int *) = {pa::read_status_loop,       pa::read_status_reduce,    pa::read_status_fp8_loop,
+                             pa::read_status_fp8_reduce, pa::read_status_int8_loop, pa::read_status_int8_reduce};
   int worst = 0;
   for (auto reader : readers) {
     int v = 0;

@@ -5,7 +5,8 @@
 // in the layout the attention kernels read, [num_blocks, block_size, num_kv_heads, head_size]
 // (paged_attention_kernel_loop.hpp:50-51).  This kernel defines the same contract on the
 // device: value stored = round-to-nearest-even(x / scale) in e5m2 or e4m3 (saturating to
-// the largest finite code), or x itself for an fp16 cache.  The scale is fp8_scale, or the
+// the largest finite code), the nearest integer in -127 .. 127 (ties to even) for an int8 cache, or x
+// itself for an fp16 cache.  The scale is fp8_scale, or the
 // entry of the token's KV head (and block) in the per-head / per-block scale arrays that the
 // attention entry points read back under the same names.
 #include <cuda_fp16.h>
@@ -20,6 +21,12 @@ namespace pa {
 // 8 fp16 values (one 16-byte load) -> 8 cache elements
 // `exact_rcp` != 0 means 1 / scale is a power of two, so multiplying by it is exact and
 // equals the division bit for bit; otherwise an IEEE division keeps the torch arithmetic.
+// One value over its scale -> the nearest integer of -127 .. 127 (ties to even; NaN -> 0).  -128 stays
+// unused so that the codes are symmetric.
+__device__ __forceinline__ uint32_t int8_code(float x) {
+  return static_cast<uint32_t>(max(-127, min(127, __float2int_rn(x)))) & 0xffu;
+}
+
 template <int KV>
 __device__ __forceinline__ void store_converted(void *dst_row, uint32_t elem, uint4 v, float scale,
                                                 float exact_rcp) {
@@ -41,9 +48,13 @@ __device__ __forceinline__ void store_converted(void *dst_row, uint32_t elem, ui
         a.x = __fdiv_rn(a.x, scale); a.y = __fdiv_rn(a.y, scale);
         b.x = __fdiv_rn(b.x, scale); b.y = __fdiv_rn(b.y, scale);
       }
-      const uint32_t lo = __nv_cvt_float2_to_fp8x2(a, __NV_SATFINITE, fmt);
-      const uint32_t hi = __nv_cvt_float2_to_fp8x2(b, __NV_SATFINITE, fmt);
-      packed[i] = lo | (hi << 16);
+      if constexpr (KV == KV_I8) {
+        packed[i] = int8_code(a.x) | (int8_code(a.y) << 8) | (int8_code(b.x) << 16) | (int8_code(b.y) << 24);
+      } else {
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(a, __NV_SATFINITE, fmt);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(b, __NV_SATFINITE, fmt);
+        packed[i] = lo | (hi << 16);
+      }
     }
     *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(dst_row) + elem) = make_uint2(packed[0], packed[1]);
   }
@@ -108,7 +119,8 @@ reshape_and_cache_kernel(const __half *__restrict__ key, const __half *__restric
 extern "C" PA_API int pa_reshape_and_cache(const pa_cache_write_params *p, void *stream) {
   using namespace pa;
   if (p == nullptr) return fail(PA_ERR_BAD_ARG, "params is null");
-  if (p->kv_dtype != PA_KV_F16 && p->kv_dtype != PA_KV_FP8_E5M2 && p->kv_dtype != PA_KV_FP8_E4M3)
+  if (p->kv_dtype != PA_KV_F16 && p->kv_dtype != PA_KV_FP8_E5M2 && p->kv_dtype != PA_KV_FP8_E4M3 &&
+      p->kv_dtype != PA_KV_INT8)
     return fail(PA_ERR_BAD_ARG, "unknown kv_dtype %d", p->kv_dtype);
   if (p->num_tokens == 0) return PA_OK;
   if (!p->key || !p->value || !p->key_cache || !p->value_cache || !p->slot_mapping)
@@ -125,7 +137,7 @@ extern "C" PA_API int pa_reshape_and_cache(const pa_cache_write_params *p, void 
     return fail(PA_ERR_BAD_ARG, "k_scale_per_block and v_scale_per_block must be given together");
   if (per_head && per_block) return fail(PA_ERR_BAD_ARG, "per-head and per-block scales exclude each other");
   if ((per_head || per_block) && p->kv_dtype == PA_KV_F16)
-    return fail(PA_ERR_BAD_ARG, "scale arrays need an FP8 cache");
+    return fail(PA_ERR_BAD_ARG, "scale arrays need an FP8 or int8 cache");
   if ((per_head || per_block) && (p->head_size == 0 || p->head_size % 8 != 0))
     return fail(PA_ERR_BAD_ARG, "scale arrays need a head_size that is a multiple of 8");
   if (p->kv_dtype != PA_KV_F16 && !per_head && !per_block && !(p->fp8_scale > 0.f))
@@ -166,7 +178,7 @@ extern "C" PA_API int pa_reshape_and_cache(const pa_cache_write_params *p, void 
   using kernel_fn = void (*)(const __half *, const __half *, void *, void *, const int64_t *, uint32_t, uint64_t,
                              float, float, ScaleArrays);
   // [cache type][chained][scale kind]; an fp16 cache has no scales
-  static const kernel_fn table[3][2][3] = {
+  static const kernel_fn table[4][2][3] = {
       {{reshape_and_cache_kernel<KV_F16, false, SCALE_SCALAR>, nullptr, nullptr},
        {reshape_and_cache_kernel<KV_F16, true, SCALE_SCALAR>, nullptr, nullptr}},
       {{reshape_and_cache_kernel<KV_E5M2, false, SCALE_SCALAR>, reshape_and_cache_kernel<KV_E5M2, false, SCALE_PER_HEAD>,
@@ -176,8 +188,12 @@ extern "C" PA_API int pa_reshape_and_cache(const pa_cache_write_params *p, void 
       {{reshape_and_cache_kernel<KV_E4M3, false, SCALE_SCALAR>, reshape_and_cache_kernel<KV_E4M3, false, SCALE_PER_HEAD>,
         reshape_and_cache_kernel<KV_E4M3, false, SCALE_PER_BLOCK>},
        {reshape_and_cache_kernel<KV_E4M3, true, SCALE_SCALAR>, reshape_and_cache_kernel<KV_E4M3, true, SCALE_PER_HEAD>,
-        reshape_and_cache_kernel<KV_E4M3, true, SCALE_PER_BLOCK>}}};
-  const int type_index = (p->kv_dtype == PA_KV_F16) ? 0 : (p->kv_dtype == PA_KV_FP8_E5M2) ? 1 : 2;
+        reshape_and_cache_kernel<KV_E4M3, true, SCALE_PER_BLOCK>}},
+      {{reshape_and_cache_kernel<KV_I8, false, SCALE_SCALAR>, reshape_and_cache_kernel<KV_I8, false, SCALE_PER_HEAD>,
+        reshape_and_cache_kernel<KV_I8, false, SCALE_PER_BLOCK>},
+       {reshape_and_cache_kernel<KV_I8, true, SCALE_SCALAR>, reshape_and_cache_kernel<KV_I8, true, SCALE_PER_HEAD>,
+        reshape_and_cache_kernel<KV_I8, true, SCALE_PER_BLOCK>}}};
+  const int type_index = static_cast<int>(p->kv_dtype);
   const int scale_kind = per_head ? SCALE_PER_HEAD : per_block ? SCALE_PER_BLOCK : SCALE_SCALAR;
   const kernel_fn kernel = table[type_index][chained ? 1 : 0][scale_kind];
   PA_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, k, v, p->key_cache, p->value_cache, p->slot_mapping, re,

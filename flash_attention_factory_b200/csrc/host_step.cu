@@ -16,6 +16,8 @@ int launch_entry(int32_t entry, const pa_params *p, void *stream) {
   case PA_ENTRY_LOOP: return launch_kernels_loop(p, stream, nullptr);
   case PA_ENTRY_REDUCE: return launch_kernels_reduce(p, stream, nullptr);
   case PA_ENTRY_FP8_LOOP: return launch_kernels_fp8_loop(p, stream, nullptr);
+  case PA_ENTRY_INT8_LOOP: return launch_kernels_int8_loop(p, stream, nullptr);
+  case PA_ENTRY_INT8_REDUCE: return launch_kernels_int8_reduce(p, stream, nullptr);
   default: return launch_kernels_fp8_reduce(p, stream, nullptr);
   }
 }
@@ -141,7 +143,7 @@ PA_API int pa_split_by_kv_length(const uint32_t *context_lens, uint32_t num_seqs
 PA_API int pa_decode_step_host(int32_t entry, const pa_params *p, const pa_host_step *io, void *stream,
                                int32_t synchronize) {
   if (p == nullptr || io == nullptr) return pa::fail(PA_ERR_BAD_ARG, "params or host step is null");
-  if (entry < PA_ENTRY_LOOP || entry > PA_ENTRY_FP8_REDUCE) return pa::fail(PA_ERR_BAD_ARG, "unknown entry %d", entry);
+  if (entry < PA_ENTRY_LOOP || entry > PA_ENTRY_INT8_REDUCE) return pa::fail(PA_ERR_BAD_ARG, "unknown entry %d", entry);
   if ((io->in_bytes != 0 && (io->host_in == nullptr || io->dev_in == nullptr)) ||
       (io->out_bytes != 0 && io->host_out == nullptr))
     return pa::fail(PA_ERR_BAD_ARG, "host step: a buffer with a non-zero size is null");
@@ -177,7 +179,7 @@ PA_API int pa_decode_step_host_batch(int32_t entry, const pa_params *p, const pa
                                      int32_t synchronize) {
   using namespace pa;
   if (p == nullptr || io == nullptr) return fail(PA_ERR_BAD_ARG, "params or host batch is null");
-  if (entry < PA_ENTRY_LOOP || entry > PA_ENTRY_FP8_REDUCE) return fail(PA_ERR_BAD_ARG, "unknown entry %d", entry);
+  if (entry < PA_ENTRY_LOOP || entry > PA_ENTRY_INT8_REDUCE) return fail(PA_ERR_BAD_ARG, "unknown entry %d", entry);
   if (p->seq_indices != nullptr)
     return fail(PA_ERR_BAD_ARG, "host batch: sub-batches are ranges of consecutive sequences, seq_indices must be NULL");
   const uint32_t S = p->num_seqs;
@@ -189,7 +191,7 @@ PA_API int pa_decode_step_host_batch(int32_t entry, const pa_params *p, const pa
   if (packed != (p->block_table_offsets != nullptr))
     return fail(PA_ERR_BAD_ARG, "host batch: host and device block-table offsets must both be set or both be NULL");
   if (io->sub_batches > kMaxSubBatches) return fail(PA_ERR_BAD_ARG, "host batch: at most %u sub-batches", kMaxSubBatches);
-  const bool reduce = entry == PA_ENTRY_REDUCE || entry == PA_ENTRY_FP8_REDUCE;
+  const bool reduce = entry == PA_ENTRY_REDUCE || entry == PA_ENTRY_FP8_REDUCE || entry == PA_ENTRY_INT8_REDUCE;
   const size_t row_bytes = static_cast<size_t>(p->num_heads) * p->head_size * 2; // one sequence of query / out
   const size_t table_entries = table_entries_of(p, io);
   const uint32_t n = choose_sub_batches(p, io);

@@ -109,9 +109,9 @@ int encode_cache_map(CUtensorMap *map, const void *cache, const pa_params *p, ui
 // ----------------------------------------------------------------- validation
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// Checks shared by all entry points.  `fp8_entry` selects which kv_dtype values
-// the entry point accepts; `needs_scratch` is true for the split variant.
-inline int validate_params(const pa_params *p, bool fp8_entry, bool needs_scratch) {
+// Checks shared by all entry points.  `fp8_entry` (an 8-bit cache; `int8_entry`: of integers) selects which
+// kv_dtype values the entry point accepts; `needs_scratch` is true for the split variant.
+inline int validate_params(const pa_params *p, bool fp8_entry, bool needs_scratch, bool int8_entry = false) {
   if (p == nullptr) return fail(PA_ERR_BAD_ARG, "params is null");
   // the two checks the reference makes, with its messages
   // (launch_kernels_loop.h:114-115,170-172)
@@ -121,7 +121,10 @@ inline int validate_params(const pa_params *p, bool fp8_entry, bool needs_scratc
   if (!head_ok || !block_ok) return fail(PA_ERR_UNSUPPORTED, "Unsupported head size or block size");
   if (p->num_queries_per_tokens < 1 || p->num_queries_per_tokens > 8)
     return fail(PA_ERR_UNSUPPORTED, "Unsupported number of queries per token");
-  if (fp8_entry) {
+  if (int8_entry) {
+    if (p->kv_dtype != PA_KV_INT8)
+      return fail(PA_ERR_BAD_ARG, "int8 entry point needs kv_dtype int8, got %d", p->kv_dtype);
+  } else if (fp8_entry) {
     if (p->kv_dtype != PA_KV_FP8_E5M2 && p->kv_dtype != PA_KV_FP8_E4M3)
       return fail(PA_ERR_BAD_ARG, "FP8 entry point needs kv_dtype e5m2 or e4m3, got %d", p->kv_dtype);
   } else if (p->kv_dtype != PA_KV_F16) {

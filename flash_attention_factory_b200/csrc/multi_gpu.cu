@@ -54,6 +54,8 @@ int default_launch(int32_t entry, const pa_params *p, void *stream, void *) {
   case PA_ENTRY_REDUCE: return launch_kernels_reduce(p, stream, nullptr);
   case PA_ENTRY_FP8_LOOP: return launch_kernels_fp8_loop(p, stream, nullptr);
   case PA_ENTRY_FP8_REDUCE: return launch_kernels_fp8_reduce(p, stream, nullptr);
+  case PA_ENTRY_INT8_LOOP: return launch_kernels_int8_loop(p, stream, nullptr);
+  case PA_ENTRY_INT8_REDUCE: return launch_kernels_int8_reduce(p, stream, nullptr);
   default: return fail(PA_ERR_BAD_ARG, "unknown entry %d", entry);
   }
 }

@@ -8,8 +8,9 @@
 //   MODE_SPLIT  persistent CTAs walking (sequence, partition, KV-head group) items;
 //               writes max_logits, exp_sums and the fp16 partial output
 //               (reference paged_attention_kernel, paged_attention_kernel_v2.hpp:42-588)
-// with the KV cache stored as fp16, e5m2 or e4m3 (FP8 dequantised in
-// registers, reference paged_attention_kernel_fp8_loop.hpp:270-278,328-333,540-545).
+// with the KV cache stored as fp16, e5m2, e4m3 (FP8 dequantised in
+// registers, reference paged_attention_kernel_fp8_loop.hpp:270-278,328-333,540-545) or 8-bit
+// integers.
 // merge_partitions_kernel is the second kernel of the split variant
 // (reference paged_attention_reduce, paged_attention_kernel_v2.hpp:594-970).
 //
@@ -165,6 +166,9 @@ struct AttnArgs {
   // context of a (sequence, head group), its normalised result goes straight to `out`, and the
   // scratch tensors are neither read nor written (they may be null)
   uint32_t whole_context_items;
+  // split mode: the last partition that the scratch has room for runs to the end of the context,
+  // whatever its length (differential attention, whose partition size follows from the scratch)
+  uint32_t last_partition_open;
   // max_blocks_per_seq * block_size (saturated to 32 bits): a context length beyond it is cut
   // to it, so no block-table read leaves the sequence's row whatever context_lens holds
   uint32_t ctx_limit;
@@ -191,7 +195,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // the rescaling of the accumulator.
 constexpr float kRescaleThreshold = 8.0f;
 
-template <int D, int KV, int NWARPS = 4, int TILES = 1>
+template <int D, int KV, int NWARPS = 4, int TILES = 1, int VH = 1>
 struct SmemLayout {
   using policy = paged_attention_policy_v2<D, KV, NWARPS, TILES>;
   using geo = typename policy::geometry;
@@ -204,9 +208,9 @@ struct SmemLayout {
   static constexpr uint32_t STAGE_BYTES = 2 * KV_TILE;
   static constexpr uint32_t RING_BYTES = NSTAGES * STAGE_BYTES;
   static_assert(NW == 4 || NW == 8, "warp <-> (head, token slice) mapping: 4 warps, or 8 with one head per warp");
-  // split mode, fewer than 4 heads per CTA: two O[8][D] buffers filled in a fixed order
+  // split mode, fewer than 4 heads per CTA: two O[8][VH * D] buffers filled in a fixed order
   static constexpr uint32_t MERGE_OFFSET = RING_BYTES;
-  static constexpr uint32_t MERGE_BYTES = (NWARPS == 8) ? 0 : 2 * 8 * D * 4; // the wide CTA never merges
+  static constexpr uint32_t MERGE_BYTES = (NWARPS == 8) ? 0 : 2 * 8 * VH * D * 4; // the wide CTA never merges
   // per-warp (reference max, true max, sum) of the 8 query columns, double-buffered by item parity
   static constexpr uint32_t WARP_STATS_OFFSET = MERGE_OFFSET + MERGE_BYTES;
   static constexpr uint32_t WARP_STATS_FLOATS = 3 * NW * 8;
@@ -365,6 +369,7 @@ struct SplitCursor {
     } else {
       it.tok_begin = it.partition << args.partition_shift;
       it.tok_end = min(ctx, it.tok_begin + (1u << args.partition_shift));
+      if (args.last_partition_open != 0u && it.partition + 1u == args.max_num_partitions) it.tok_end = ctx;
     }
     it.ctx = ctx;
     it.table_off = __shfl_sync(0xffffffffu, lane_off, owner);
@@ -373,13 +378,23 @@ struct SplitCursor {
   }
 };
 
-template <int D, int KV>
+// Query head behind column g of KV head kv_head.  Ordinary attention: the group's heads are
+// neighbours.  Differential attention (VH == 2): head h of KV pair k = h / G has its two maps
+// at 2 h and 2 h + 1, and map c reads K head 2 k + c.
+template <int VH>
+__device__ __forceinline__ uint32_t query_head_of(uint32_t kv_head, uint32_t G, uint32_t g) {
+  if constexpr (VH == 1) return kv_head * G + g;
+  else return ((kv_head >> 1) * G + g) * 2u + (kv_head & 1u);
+}
+
+template <int D, int KV, int VH = 1>
 __device__ __forceinline__ void load_q_fragments(uint32_t (&qf)[D / 16][2], const AttnArgs &args,
                                                  uint32_t seq, uint32_t kv_head, uint32_t gid,
                                                  uint32_t t4) {
   // B operand of S^T = K . Q^T: column n = gid is the query head inside the group
   const uint32_t G = args.group;
-  const __half *qrow = args.query + (static_cast<size_t>(seq) * args.num_heads + kv_head * G + gid) * D;
+  const __half *qrow =
+      args.query + (static_cast<size_t>(seq) * args.num_heads + query_head_of<VH>(kv_head, G, gid)) * D;
 #pragma unroll
   for (uint32_t ks = 0; ks < D / 16; ++ks) {
     if (gid < G) {
@@ -501,13 +516,21 @@ __device__ __noinline__ void merge_cluster_rows(float *areas, __half *out, const
 // instantiation (the loop launchers also run the persistent form).  With external linkage the
 // host stubs of such twins would be merged and a launch could run the other unit's copy, with
 // the other unit's tables behind this unit's slot allocator.
+//
+// VH is the number of V heads that the weights of a K head meet: 1, or 2 in differential
+// attention, where the KV heads come in pairs (2 k, 2 k + 1), each has a query map and softmax of
+// its own, and both maps weigh the pair's two V heads side by side (a value vector of 2 D).  The
+// warp of a head then reads the V tiles of its neighbour too, which lie in the same stage: every
+// byte still comes from HBM once, the extra cost is shared-memory reads, conversions and MMAs.
+// Split mode only, hpc even; the partial rows are fp32 and twice as wide.
 namespace {
-template <int D, int KV, int MODE, int NWARPS = 4, int TILES = 1>
+template <int D, int KV, int MODE, int NWARPS = 4, int TILES = 1, int VH = 1>
 __global__ void __launch_bounds__(paged_attention_policy_v2<D, KV, NWARPS, TILES>::threads_per_cta,
                                   paged_attention_policy_v2<D, KV, NWARPS, TILES>::ctas_per_sm)
 paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
                        const __grid_constant__ CUtensorMap tmap_v, const AttnArgs args) {
-  using L = SmemLayout<D, KV, NWARPS, TILES>;
+  static_assert(VH == 1 || (VH == 2 && MODE == MODE_SPLIT), "differential attention exists in split mode only");
+  using L = SmemLayout<D, KV, NWARPS, TILES, VH>;
   using policy = typename L::policy;
   using geo = typename L::geo;
   constexpr uint32_t NW = L::NW;
@@ -532,6 +555,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
   constexpr uint32_t kNoItem = 0xffffffffu;
   float2 *stage_scales = reinterpret_cast<float2 *>(smem + L::SCALES_OFFSET); // [NSTAGES][SCALE_SLOTS]
   const bool block_scales = (KV != KV_F16) && args.k_scale_per_block != nullptr;
+  // Per-block scales of an int8 cache, and of any cache in differential attention, are folded into the
+  // straight-line path too, with a running reference for the V scales (see fold_v_scales); the FP8
+  // caches of ordinary attention keep them on the general path, where their order of operations was set.
+  constexpr bool BLOCK_FAST = (KV == KV_I8) || (VH == 2 && KV != KV_F16);
 
   const uint32_t warp = threadIdx.x >> 5;
   const uint32_t lane = threadIdx.x & 31u;
@@ -948,12 +975,86 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
 #endif
     uint32_t qf[KSTEPS][2];
     WorkItem cur = first;
-    if (cur.valid) load_q_fragments<D, KV>(qf, args, cur.seq, cur.head_base + my_head, gid, t4);
+    if (cur.valid) load_q_fragments<D, KV, VH>(qf, args, cur.seq, cur.head_base + my_head, gid, t4);
 
     // state of query columns g = 2*t4 and 2*t4+1, log2 domain: m_ref is the exponent
     // reference the weights are taken against, m_true the running maximum
     float m_ref[2], m_true[2], l_run[2];
-    float acc[KSTEPS][4];
+    float acc[VH][KSTEPS][4];
+    // first V head this warp reads, relative to its own head (rows of the stage are head-major)
+    const uint32_t v_head0 = (VH == 1) ? my_head : (my_head & ~1u);
+    const uint32_t v_shift = (v_head0 - my_head) * tps * geo::slab_bytes; // 0, or minus one head (modulo 2^32)
+    const uint32_t v_head_bytes = tps * geo::slab_bytes;
+    // O^T += V^T . P^T over the VH heads, each with its own weights
+    auto value_tiles = [&](uint32_t v_base, const uint32_t (&p_lo)[VH], const uint32_t (&p_hi)[VH]) {
+#pragma unroll
+      for (uint32_t vh = 0; vh < VH; ++vh)
+        value_tile(v_base + v_shift + vh * v_head_bytes, p_lo[vh], p_hi[vh], acc[vh]);
+    };
+    auto zero_value_tiles = [&](uint32_t v_base, uint32_t first_token, uint32_t num_rows) {
+#pragma unroll
+      for (uint32_t vh = 0; vh < VH; ++vh)
+        zero_value_rows(v_base, (v_head0 + vh) * tps + my_slice * 16 + first_token, num_rows, lane);
+    };
+    auto scale_accumulators = [&](float r0, float r1) {
+#pragma unroll
+      for (uint32_t vh = 0; vh < VH; ++vh) {
+#pragma unroll
+        for (uint32_t i = 0; i < KSTEPS; ++i) {
+          acc[vh][i][0] *= r0;
+          acc[vh][i][1] *= r1;
+          acc[vh][i][2] *= r0;
+          acc[vh][i][3] *= r1;
+        }
+      }
+    };
+    // Running reference of the V block scales (BLOCK_FAST): a tile's weights are multiplied by its
+    // scale over the largest scale so far, a factor of at most 1, before they are rounded to fp16,
+    // and the accumulator carries the reference; multiplying by the scale itself would push the
+    // weights of a cache with small values into the subnormal halves.  Uniform across the warp;
+    // the reference grows about ln(blocks) times per item.
+    float v_ref = 0.f, v_inv = 0.f;
+    auto fold_v_scales = [&](const float (&va)[VH], const float (&vb)[VH], float (&wa)[VH], float (&wb)[VH]) {
+      float top = fmaxf(va[0], vb[0]);
+      if constexpr (VH == 2) top = fmaxf(top, fmaxf(va[1], vb[1]));
+      if (top > v_ref) {
+        const float r = v_ref / top;
+        scale_accumulators(r, r);
+        v_ref = top;
+        v_inv = 1.f / top;
+      }
+#pragma unroll
+      for (uint32_t vh = 0; vh < VH; ++vh) {
+        wa[vh] = va[vh] * v_inv;
+        wb[vh] = vb[vh] * v_inv;
+      }
+    };
+    // fp16 weights of one tile as the B operand of the value product, transposed, one set per V head
+    auto pack_weights = [&](const float (&p)[4], const float (&w)[VH], bool weighted, uint32_t (&lo)[VH],
+                            uint32_t (&hi)[VH]) {
+      if (!weighted) {
+        lo[0] = movmatrix_trans(pack_half2(p[0], p[1])); // tokens 0..7
+        hi[0] = movmatrix_trans(pack_half2(p[2], p[3])); // tokens 8..15
+        if constexpr (VH == 2) {
+          lo[1] = lo[0];
+          hi[1] = hi[0];
+        }
+        return;
+      }
+#pragma unroll
+      for (uint32_t vh = 0; vh < VH; ++vh) {
+        lo[vh] = movmatrix_trans(pack_half2(p[0] * w[vh], p[1] * w[vh]));
+        hi[vh] = movmatrix_trans(pack_half2(p[2] * w[vh], p[3] * w[vh]));
+      }
+    };
+    // K scale (log2-domain softmax scale) and V scales of the tile that starts at `row` of a stage.
+    // A zero scale (a block of zeros) keeps a tiny positive softmax scale, so that -inf stays -inf.
+    auto tile_scales = [&](uint32_t stage_slot, uint32_t row, float &k_scale, float (&v)[VH]) {
+      const float2 *s = stage_scales + stage_slot * L::SCALE_SLOTS + (row / args.rows_per_box) * hpc;
+      k_scale = fmaxf(args.sm_scale_log2 * s[my_head].x, 1e-30f);
+#pragma unroll
+      for (uint32_t vh = 0; vh < VH; ++vh) v[vh] = s[v_head0 + vh].y;
+    };
 
     uint32_t item_no = 0;
     while (cur.valid) {
@@ -964,11 +1065,16 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
       const float scale = (args.k_scale_per_head != nullptr)
                               ? args.sm_scale_log2 * __ldg(args.k_scale_per_head + kv_head)
                               : args.scale_log2;
-      const float out_scale = (args.v_scale_per_head != nullptr) ? __ldg(args.v_scale_per_head + kv_head)
-                                                                 : args.out_scale;
-      // score modifiers and per-block scales take the general path below; the straight-line
+      float out_scale[VH];
+#pragma unroll
+      for (uint32_t vh = 0; vh < VH; ++vh)
+        out_scale[vh] = (args.v_scale_per_head != nullptr)
+                            ? __ldg(args.v_scale_per_head + cur.head_base + v_head0 + vh)
+                            : args.out_scale;
+      // score modifiers and per-block FP8 scales take the general path below; the straight-line
       // path for pairs of full tiles is for the plain case only
-      const bool modifiers = (args.alibi_slopes != nullptr) || (args.softcap > 0.f) || block_scales;
+      const bool modifiers =
+          (args.alibi_slopes != nullptr) || (args.softcap > 0.f) || (block_scales && !BLOCK_FAST);
       float slope[2] = {0.f, 0.f}; // ALiBi slopes of query columns 2*t4, 2*t4+1
       if (args.alibi_slopes != nullptr) {
 #pragma unroll
@@ -979,7 +1085,11 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
       m_ref[0] = m_ref[1] = m_true[0] = m_true[1] = neg_infinity();
       l_run[0] = l_run[1] = 0.f; // per-lane partial sums; reduced over gid at the end
 #pragma unroll
-      for (uint32_t i = 0; i < KSTEPS; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+      for (uint32_t vh = 0; vh < VH; ++vh) {
+#pragma unroll
+        for (uint32_t i = 0; i < KSTEPS; ++i) acc[vh][i][0] = acc[vh][i][1] = acc[vh][i][2] = acc[vh][i][3] = 0.f;
+      }
+      v_ref = v_inv = 0.f;
       // The sink is one extra logit with a zero value vector, attached to the first tokens
       // of the context only (reference paged_attention_kernel_loop.hpp:387-401).
       if (args.sinks != nullptr && my_slice == 0 && cur.tok_begin == 0) {
@@ -1046,8 +1156,21 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
           // to the rescale test; every value is computed as in the general case below
           float ca[4], cb[4];
           score_tile_pair(base_a + lm_off_a, base_b + lm_off_a, qf, ca, cb);
-          m_true[0] = fmaxf(m_true[0], quad_column_max(fmaxf(fmaxf(ca[0], ca[2]), fmaxf(cb[0], cb[2]))) * scale);
-          m_true[1] = fmaxf(m_true[1], quad_column_max(fmaxf(fmaxf(ca[1], ca[3]), fmaxf(cb[1], cb[3]))) * scale);
+          float s_a = scale, s_b = scale; // softmax scales of the two tiles
+          float w_a[VH], w_b[VH];         // V scales of the two tiles over the reference
+          if constexpr (BLOCK_FAST) {
+            if (block_scales) {
+              float v_a[VH], v_b[VH];
+              tile_scales(slot_a, sub_a * tpt + my_slice * 16u, s_a, v_a);
+              tile_scales(slot_b, sub_b * tpt + my_slice * 16u, s_b, v_b);
+              fold_v_scales(v_a, v_b, w_a, w_b);
+            }
+            m_true[0] = fmaxf(m_true[0], quad_column_max(fmaxf(fmaxf(ca[0], ca[2]) * s_a, fmaxf(cb[0], cb[2]) * s_b)));
+            m_true[1] = fmaxf(m_true[1], quad_column_max(fmaxf(fmaxf(ca[1], ca[3]) * s_a, fmaxf(cb[1], cb[3]) * s_b)));
+          } else {
+            m_true[0] = fmaxf(m_true[0], quad_column_max(fmaxf(fmaxf(ca[0], ca[2]), fmaxf(cb[0], cb[2]))) * scale);
+            m_true[1] = fmaxf(m_true[1], quad_column_max(fmaxf(fmaxf(ca[1], ca[3]), fmaxf(cb[1], cb[3]))) * scale);
+          }
           const bool stale = (m_true[0] > m_ref[0] + kRescaleThreshold) ||
                              (m_true[1] > m_ref[1] + kRescaleThreshold);
           if (__any_sync(0xffffffffu, stale)) {
@@ -1055,41 +1178,35 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
             const float r1 = (m_ref[1] == neg_infinity()) ? 0.f : fast_exp2(m_ref[1] - m_true[1]);
             l_run[0] *= r0;
             l_run[1] *= r1;
-#pragma unroll
-            for (uint32_t i = 0; i < KSTEPS; ++i) {
-              acc[i][0] *= r0;
-              acc[i][1] *= r1;
-              acc[i][2] *= r0;
-              acc[i][3] *= r1;
-            }
+            scale_accumulators(r0, r1);
             m_ref[0] = m_true[0];
             m_ref[1] = m_true[1];
           }
           float pa[4], pb[4];
 #pragma unroll
           for (uint32_t j = 0; j < 4; ++j) {
-            pa[j] = fast_exp2(fmaf(ca[j], scale, -m_ref[j & 1u]));
-            pb[j] = fast_exp2(fmaf(cb[j], scale, -m_ref[j & 1u]));
+            pa[j] = fast_exp2(fmaf(ca[j], s_a, -m_ref[j & 1u]));
+            pb[j] = fast_exp2(fmaf(cb[j], s_b, -m_ref[j & 1u]));
           }
           l_run[0] += (pa[0] + pa[2]) + (pb[0] + pb[2]);
           l_run[1] += (pa[1] + pa[3]) + (pb[1] + pb[3]);
-          const uint32_t pa_lo = movmatrix_trans(pack_half2(pa[0], pa[1]));
-          const uint32_t pa_hi = movmatrix_trans(pack_half2(pa[2], pa[3]));
-          const uint32_t pb_lo = movmatrix_trans(pack_half2(pb[0], pb[1]));
-          const uint32_t pb_hi = movmatrix_trans(pack_half2(pb[2], pb[3]));
-          value_tile(base_a + L::KV_TILE, pa_lo, pa_hi, acc);
+          uint32_t pa_lo[VH], pa_hi[VH], pb_lo[VH], pb_hi[VH];
+          const bool weighted = BLOCK_FAST && block_scales;
+          pack_weights(pa, w_a, weighted, pa_lo, pa_hi);
+          pack_weights(pb, w_b, weighted, pb_lo, pb_hi);
+          value_tiles(base_a + L::KV_TILE, pa_lo, pa_hi);
           if constexpr (TILES == 1) {
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty_bar[slot_a]); // stage A goes back before stage B is used
             released_a = true;
           }
-          value_tile(base_b + L::KV_TILE, pb_lo, pb_hi, acc);
+          value_tiles(base_b + L::KV_TILE, pb_lo, pb_hi);
         } else if (alive && tok_a < my_tokens) {
           const bool act_b = has_b && tok_b < my_tokens;
           const uint32_t n_a = min(16u, my_tokens - tok_a);
           const uint32_t n_b = act_b ? min(16u, my_tokens - tok_b) : 0u;
-          if (n_a < 16u) zero_value_rows(base_a + L::KV_TILE, warp_row + n_a, 16u - n_a, lane);
-          if (act_b && n_b < 16u) zero_value_rows(base_b + L::KV_TILE, warp_row + n_b, 16u - n_b, lane);
+          if (n_a < 16u) zero_value_tiles(base_a + L::KV_TILE, n_a, 16u - n_a);
+          if (act_b && n_b < 16u) zero_value_tiles(base_b + L::KV_TILE, n_b, 16u - n_b);
 
           // ---- S^T = K . Q^T ; lane holds S[tok gid][g 2t4, 2t4+1] in [0],[1] and
           // S[tok gid+8][..] in [2],[3]
@@ -1103,7 +1220,21 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
           float eff_scale = scale;
           float v_scale_a = 1.f, v_scale_b = 1.f; // per-block V scales of the two tiles
           float k_nat_a = scale * kLn2, k_nat_b = scale * kLn2; // sm_scale * k scale of the two tiles
-          if (block_scales) {
+          float s_a = scale, s_b = scale; // BLOCK_FAST: softmax scales of the two tiles,
+          float w_a[VH], w_b[VH];         // and their V scales over the reference
+          if constexpr (BLOCK_FAST) {
+            if (block_scales) {
+              float v_a[VH], v_b[VH];
+              tile_scales(slot_a, sub_a * tpt + my_slice * 16u, s_a, v_a);
+              s_b = s_a;
+#pragma unroll
+              for (uint32_t vh = 0; vh < VH; ++vh) v_b[vh] = 0.f;
+              if (act_b) tile_scales(slot_b, sub_b * tpt + my_slice * 16u, s_b, v_b);
+              fold_v_scales(v_a, v_b, w_a, w_b);
+              k_nat_a = s_a * kLn2;
+              k_nat_b = s_b * kLn2;
+            }
+          } else if (block_scales) {
             // tile A / B lie in one KV block each: the stage's slot for (that block, this head)
             const uint32_t chunk_a = (sub_a * tpt + my_slice * 16u) / args.rows_per_box;
             const uint32_t chunk_b = (sub_b * tpt + my_slice * 16u) / args.rows_per_box;
@@ -1133,7 +1264,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
               ca[j] = xa * kLog2e;
               cb[j] = act_b ? xb * kLog2e : neg_infinity();
             }
-            eff_scale = 1.f;
+            eff_scale = s_a = s_b = 1.f;
           }
           if (modifiers || n_a < 16u || (act_b && n_b < 16u)) {
             // tokens past the context never count, whatever the cache holds there
@@ -1145,8 +1276,14 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
           }
           // ---- online softmax (reference paged_attention_kernel_loop.hpp:382-419);
           // scale > 0, so the maximum commutes with the scaling
-          m_true[0] = fmaxf(m_true[0], quad_column_max(fmaxf(fmaxf(ca[0], ca[2]), fmaxf(cb[0], cb[2]))) * eff_scale);
-          m_true[1] = fmaxf(m_true[1], quad_column_max(fmaxf(fmaxf(ca[1], ca[3]), fmaxf(cb[1], cb[3]))) * eff_scale);
+          if constexpr (BLOCK_FAST) {
+            m_true[0] = fmaxf(m_true[0], quad_column_max(fmaxf(fmaxf(ca[0], ca[2]) * s_a, fmaxf(cb[0], cb[2]) * s_b)));
+            m_true[1] = fmaxf(m_true[1], quad_column_max(fmaxf(fmaxf(ca[1], ca[3]) * s_a, fmaxf(cb[1], cb[3]) * s_b)));
+          } else {
+            s_a = s_b = eff_scale;
+            m_true[0] = fmaxf(m_true[0], quad_column_max(fmaxf(fmaxf(ca[0], ca[2]), fmaxf(cb[0], cb[2]))) * eff_scale);
+            m_true[1] = fmaxf(m_true[1], quad_column_max(fmaxf(fmaxf(ca[1], ca[3]), fmaxf(cb[1], cb[3]))) * eff_scale);
+          }
           const bool stale = (m_true[0] > m_ref[0] + kRescaleThreshold) ||
                              (m_true[1] > m_ref[1] + kRescaleThreshold);
           if (__any_sync(0xffffffffu, stale)) {
@@ -1154,25 +1291,20 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
             const float r1 = (m_ref[1] == neg_infinity()) ? 0.f : fast_exp2(m_ref[1] - m_true[1]);
             l_run[0] *= r0;
             l_run[1] *= r1;
-#pragma unroll
-            for (uint32_t i = 0; i < KSTEPS; ++i) {
-              acc[i][0] *= r0;
-              acc[i][1] *= r1;
-              acc[i][2] *= r0;
-              acc[i][3] *= r1;
-            }
+            scale_accumulators(r0, r1);
             m_ref[0] = m_true[0];
             m_ref[1] = m_true[1];
           }
           float pa[4], pb[4];
 #pragma unroll
           for (uint32_t j = 0; j < 4; ++j) {
-            pa[j] = fast_exp2(fmaf(ca[j], eff_scale, -m_ref[j & 1u]));
-            pb[j] = fast_exp2(fmaf(cb[j], eff_scale, -m_ref[j & 1u]));
+            pa[j] = fast_exp2(fmaf(ca[j], s_a, -m_ref[j & 1u]));
+            pb[j] = fast_exp2(fmaf(cb[j], s_b, -m_ref[j & 1u]));
           }
           l_run[0] += (pa[0] + pa[2]) + (pb[0] + pb[2]); // fp32 sum of the unrounded weights
           l_run[1] += (pa[1] + pa[3]) + (pb[1] + pb[3]);
-          if (block_scales) {
+          const bool weighted = BLOCK_FAST && block_scales;
+          if (block_scales && !BLOCK_FAST) {
             // V of a block dequantises as code * scale: fold the scale into the weights
 #pragma unroll
             for (uint32_t j = 0; j < 4; ++j) {
@@ -1183,9 +1315,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
           // P rounded to fp16 for the MMA, transposed into the B-operand layout;
           // ---- O^T += V^T . P^T
           {
-            const uint32_t p_lo = movmatrix_trans(pack_half2(pa[0], pa[1])); // tokens 0..7
-            const uint32_t p_hi = movmatrix_trans(pack_half2(pa[2], pa[3])); // tokens 8..15
-            value_tile(base_a + L::KV_TILE, p_lo, p_hi, acc);
+            uint32_t p_lo[VH], p_hi[VH];
+            pack_weights(pa, w_a, weighted, p_lo, p_hi);
+            value_tiles(base_a + L::KV_TILE, p_lo, p_hi);
           }
           if (TILES == 1 && has_b) {
             // stage A is no longer needed: hand it back before working on stage B
@@ -1194,9 +1326,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
             released_a = true;
           }
           if (act_b) {
-            const uint32_t p_lo = movmatrix_trans(pack_half2(pb[0], pb[1]));
-            const uint32_t p_hi = movmatrix_trans(pack_half2(pb[2], pb[3]));
-            value_tile(base_b + L::KV_TILE, p_lo, p_hi, acc);
+            uint32_t p_lo[VH], p_hi[VH];
+            pack_weights(pb, w_b, weighted, p_lo, p_hi);
+            value_tiles(base_b + L::KV_TILE, p_lo, p_hi);
           }
         }
         // this warp is done with the stages: let the producer refill them
@@ -1231,43 +1363,61 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
         ++item_no;
       }
       // Q of the next item: issued now so that the loads fly during the epilogue below
-      if (nxt.valid) load_q_fragments<D, KV>(qf, args, nxt.seq, nxt.head_base + my_head, gid, t4);
+      if (nxt.valid) load_q_fragments<D, KV, VH>(qf, args, nxt.seq, nxt.head_base + my_head, gid, t4);
 
       l_run[0] = quad_column_sum(l_run[0]);
       l_run[1] = quad_column_sum(l_run[1]);
       const bool ok = (*abort_flag == 0u);
+      // with folded V scales the accumulator is relative to this warp's reference scale
+      const float acc_scale = (BLOCK_FAST && block_scales) ? v_ref : 1.f;
 
       if constexpr (MODE == MODE_SPLIT) {
         if (hpc == NW) {
           // ---- one warp per KV head: the warp holds the whole partition, write it out
           // (max_logits / exp_sums / tmp_out, reference paged_attention_kernel_v2.hpp:425-442,532-546)
-          const size_t head0 = static_cast<size_t>(cur.seq) * args.num_heads + kv_head * G;
+          const size_t seq_head = static_cast<size_t>(cur.seq) * args.num_heads;
           const bool whole = args.whole_context_items != 0u;
 #pragma unroll
           for (uint32_t j = 0; j < 2; ++j) {
             const uint32_t g = 2 * t4 + j;
             if (g < G && ok) {
-              const size_t pidx = (head0 + g) * args.max_num_partitions + cur.partition;
+              const size_t head = seq_head + query_head_of<VH>(kv_head, G, g);
+              const size_t pidx = head * args.max_num_partitions + cur.partition;
               // report the true maximum; the sum is re-expressed relative to it
               const float l_true = l_run[j] * fast_exp2(m_ref[j] - m_true[j]);
               // normalised inside the partition (reference paged_attention_kernel_v2.hpp:386);
               // a whole-context item is the final result and goes to its row of `out`
-              const float inv = (l_run[j] > 0.f) ? (out_scale / l_run[j]) : 0.f;
-              __half *dst = whole ? args.out + (head0 + g) * D : args.tmp_out + pidx * D;
-              if constexpr (KV == KV_F16) {
+              if constexpr (VH == 1) {
+                const float inv = (l_run[j] > 0.f) ? (out_scale[0] * acc_scale / l_run[j]) : 0.f;
+                __half *dst = whole ? args.out + head * D : args.tmp_out + pidx * D;
+                if constexpr (KV == KV_F16) {
 #pragma unroll
-                for (uint32_t i = 0; i < KSTEPS; ++i) {
-                  dst[i * 16 + gid] = __float2half_rn(acc[i][j] * inv);
-                  dst[i * 16 + 8 + gid] = __float2half_rn(acc[i][2 + j] * inv);
+                  for (uint32_t i = 0; i < KSTEPS; ++i) {
+                    dst[i * 16 + gid] = __float2half_rn(acc[0][i][j] * inv);
+                    dst[i * 16 + 8 + gid] = __float2half_rn(acc[0][i][2 + j] * inv);
+                  }
+                } else {
+#pragma unroll
+                  for (uint32_t q = 0; q < KSTEPS / 2; ++q) {
+                    // even/odd tiles hold neighbouring dims: one 4-byte store per pair
+                    *reinterpret_cast<uint32_t *>(dst + q * 32 + 2 * gid) =
+                        pack_half2(acc[0][2 * q][j] * inv, acc[0][2 * q + 1][j] * inv);
+                    *reinterpret_cast<uint32_t *>(dst + q * 32 + 16 + 2 * gid) =
+                        pack_half2(acc[0][2 * q][2 + j] * inv, acc[0][2 * q + 1][2 + j] * inv);
+                  }
                 }
               } else {
+                // the difference of the maps cancels, so their partial rows stay in fp32
+                float *dst = reinterpret_cast<float *>(args.tmp_out) + pidx * (VH * D);
 #pragma unroll
-                for (uint32_t q = 0; q < KSTEPS / 2; ++q) {
-                  // even/odd tiles hold neighbouring dims: one 4-byte store per pair
-                  *reinterpret_cast<uint32_t *>(dst + q * 32 + 2 * gid) =
-                      pack_half2(acc[2 * q][j] * inv, acc[2 * q + 1][j] * inv);
-                  *reinterpret_cast<uint32_t *>(dst + q * 32 + 16 + 2 * gid) =
-                      pack_half2(acc[2 * q][2 + j] * inv, acc[2 * q + 1][2 + j] * inv);
+                for (uint32_t vh = 0; vh < VH; ++vh) {
+                  const float inv = (l_run[j] > 0.f) ? (out_scale[vh] * acc_scale / l_run[j]) : 0.f;
+#pragma unroll
+                  for (uint32_t i = 0; i < KSTEPS; ++i) {
+#pragma unroll
+                    for (uint32_t h = 0; h < 2; ++h)
+                      dst[vh * D + acc_dim_index<KV>(i, h, gid)] = acc[vh][i][2 * h + j] * inv;
+                  }
                 }
               }
               if (gid == 0 && !whole) {
@@ -1299,39 +1449,46 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
           for (uint32_t j = 0; j < 2; ++j) {
             float m_all = neg_infinity();
             for (uint32_t w = w0; w < w0 + slices; ++w) m_all = fmaxf(m_all, st_ref[w * 8 + 2 * t4 + j]);
-            f[j] = (m_ref[j] == neg_infinity()) ? 0.f : fast_exp2(m_ref[j] - m_all);
+            f[j] = (m_ref[j] == neg_infinity()) ? 0.f : fast_exp2(m_ref[j] - m_all) * acc_scale;
           }
           // hpc = 1: slices 0,1 store into buffers 0,1 and slices 2,3 add to them;
           // hpc = 2: buffer = head, slice 0 stores and slice 1 adds
           const uint32_t buf_id = (hpc == 1) ? (my_slice & 1u) : my_head;
           const uint32_t round = (hpc == 1) ? (my_slice >> 1) : my_slice;
-          float *buf = merge_buf + buf_id * (8 * D);
+          constexpr uint32_t ROW = VH * D; // floats of a buffer row
+          float *buf = merge_buf + buf_id * (8 * ROW);
           if (round == 0) {
 #pragma unroll
-            for (uint32_t i = 0; i < KSTEPS; ++i) {
+            for (uint32_t vh = 0; vh < VH; ++vh) {
 #pragma unroll
-              for (uint32_t h = 0; h < 2; ++h) {
-                const uint32_t d = acc_dim_index<KV>(i, h, gid);
-                buf[(2 * t4) * D + d] = acc[i][2 * h] * f[0];
-                buf[(2 * t4 + 1) * D + d] = acc[i][2 * h + 1] * f[1];
+              for (uint32_t i = 0; i < KSTEPS; ++i) {
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h) {
+                  const uint32_t d = vh * D + acc_dim_index<KV>(i, h, gid);
+                  buf[(2 * t4) * ROW + d] = acc[vh][i][2 * h] * f[0];
+                  buf[(2 * t4 + 1) * ROW + d] = acc[vh][i][2 * h + 1] * f[1];
+                }
               }
             }
           }
           named_barrier_sync(1, NCONS);
           if (round == 1) {
 #pragma unroll
-            for (uint32_t i = 0; i < KSTEPS; ++i) {
+            for (uint32_t vh = 0; vh < VH; ++vh) {
 #pragma unroll
-              for (uint32_t h = 0; h < 2; ++h) {
-                const uint32_t d = acc_dim_index<KV>(i, h, gid);
-                buf[(2 * t4) * D + d] += acc[i][2 * h] * f[0];
-                buf[(2 * t4 + 1) * D + d] += acc[i][2 * h + 1] * f[1];
+              for (uint32_t i = 0; i < KSTEPS; ++i) {
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h) {
+                  const uint32_t d = vh * D + acc_dim_index<KV>(i, h, gid);
+                  buf[(2 * t4) * ROW + d] += acc[vh][i][2 * h] * f[0];
+                  buf[(2 * t4 + 1) * ROW + d] += acc[vh][i][2 * h + 1] * f[1];
+                }
               }
             }
           }
           named_barrier_sync(1, NCONS);
           // write out: thread -> (head, query column g, 8 consecutive dims)
-          constexpr uint32_t THREADS_PER_ROW = D / 8;
+          constexpr uint32_t THREADS_PER_ROW = ROW / 8;
           for (uint32_t idx = ctid; idx < hpc * 8 * THREADS_PER_ROW; idx += NCONS) {
             const uint32_t hh = idx / (8 * THREADS_PER_ROW);
             const uint32_t g = (idx / THREADS_PER_ROW) % 8;
@@ -1347,30 +1504,37 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
               const float mw = st_ref[w * 8 + g];
               l_all += (mw == neg_infinity()) ? 0.f : fast_exp2(mw - mr_all) * st_sum[w * 8 + g];
             }
-            const float *b0 = merge_buf + ((hpc == 1) ? 0u : hh) * (8 * D) + g * D + d0;
+            const float *b0 = merge_buf + ((hpc == 1) ? 0u : hh) * (8 * ROW) + g * ROW + d0;
             float4 lo = *reinterpret_cast<const float4 *>(b0);
             float4 hi = *reinterpret_cast<const float4 *>(b0 + 4);
             if (hpc == 1) {
-              const float4 lo1 = *reinterpret_cast<const float4 *>(b0 + 8 * D);
-              const float4 hi1 = *reinterpret_cast<const float4 *>(b0 + 8 * D + 4);
+              const float4 lo1 = *reinterpret_cast<const float4 *>(b0 + 8 * ROW);
+              const float4 hi1 = *reinterpret_cast<const float4 *>(b0 + 8 * ROW + 4);
               lo.x += lo1.x; lo.y += lo1.y; lo.z += lo1.z; lo.w += lo1.w;
               hi.x += hi1.x; hi.y += hi1.y; hi.z += hi1.z; hi.w += hi1.w;
             }
             if (g < G && ok) {
-              const size_t head = static_cast<size_t>(cur.seq) * args.num_heads + (cur.head_base + hh) * G + g;
+              const size_t head =
+                  static_cast<size_t>(cur.seq) * args.num_heads + query_head_of<VH>(cur.head_base + hh, G, g);
               const size_t pidx = head * args.max_num_partitions + cur.partition;
-              const float head_scale = (args.v_scale_per_head != nullptr)
-                                           ? __ldg(args.v_scale_per_head + cur.head_base + hh)
-                                           : args.out_scale;
+              const uint32_t v_head = cur.head_base + ((VH == 1) ? hh : (hh & ~1u) + d0 / D); // of these dims
+              const float head_scale =
+                  (args.v_scale_per_head != nullptr) ? __ldg(args.v_scale_per_head + v_head) : args.out_scale;
               const float inv = (l_all > 0.f) ? (head_scale / l_all) : 0.f;
-              uint4 packed;
-              packed.x = pack_half2(lo.x * inv, lo.y * inv);
-              packed.y = pack_half2(lo.z * inv, lo.w * inv);
-              packed.z = pack_half2(hi.x * inv, hi.y * inv);
-              packed.w = pack_half2(hi.z * inv, hi.w * inv);
               const bool whole = args.whole_context_items != 0u;
-              __half *dst = whole ? args.out + head * D : args.tmp_out + pidx * D;
-              *reinterpret_cast<uint4 *>(dst + d0) = packed;
+              if constexpr (VH == 1) {
+                uint4 packed;
+                packed.x = pack_half2(lo.x * inv, lo.y * inv);
+                packed.y = pack_half2(lo.z * inv, lo.w * inv);
+                packed.z = pack_half2(hi.x * inv, hi.y * inv);
+                packed.w = pack_half2(hi.z * inv, hi.w * inv);
+                __half *dst = whole ? args.out + head * D : args.tmp_out + pidx * D;
+                *reinterpret_cast<uint4 *>(dst + d0) = packed;
+              } else {
+                float4 *dst = reinterpret_cast<float4 *>(reinterpret_cast<float *>(args.tmp_out) + pidx * ROW + d0);
+                dst[0] = make_float4(lo.x * inv, lo.y * inv, lo.z * inv, lo.w * inv);
+                dst[1] = make_float4(hi.x * inv, hi.y * inv, hi.z * inv, hi.w * inv);
+              }
               if (d0 == 0 && !whole) {
                 args.max_logits[pidx] = mt_all * kLn2;
                 args.exp_sums[pidx] = l_all * fast_exp2(mr_all - mt_all);
@@ -1394,8 +1558,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
 #pragma unroll
           for (uint32_t h = 0; h < 2; ++h) {
             const uint32_t d = acc_dim_index<KV>(i, h, gid);
-            area[(2 * t4) * D + d] = acc[i][2 * h];
-            area[(2 * t4 + 1) * D + d] = acc[i][2 * h + 1];
+            area[(2 * t4) * D + d] = acc[0][i][2 * h] * acc_scale;
+            area[(2 * t4 + 1) * D + d] = acc[0][i][2 * h + 1] * acc_scale;
           }
         }
       }

@@ -18,7 +18,10 @@ def _require(cond: bool, msg: str) -> None:
         raise RuntimeError(msg)
 
 
-def _kv_dtype_of(cache: torch.Tensor, fp8: bool) -> int:
+def _kv_dtype_of(cache: torch.Tensor, fp8: bool, int8: bool = False) -> int:
+    if int8:
+        _require(cache.dtype == torch.int8, f"key/value cache must be int8, got {cache.dtype}")
+        return _cabi.KV_INT8
     if not fp8:
         _require(cache.dtype == torch.float16, f"key/value cache must be float16, got {cache.dtype}")
         return _cabi.KV_F16
@@ -36,11 +39,12 @@ def build_params(max_logits, exp_sums, tem_output, output, debug_output, query, 
                  fp8_scale, block_size, max_context_len, alibi_slopes, sinks, softcap,
                  fp8: bool, k_scale_per_head=None, v_scale_per_head=None,
                  use_alibi: bool = False, use_softcap: bool = False,
-                 k_scale_per_block=None, v_scale_per_block=None) -> _cabi.PaParams:
+                 k_scale_per_block=None, v_scale_per_block=None, int8: bool = False) -> _cabi.PaParams:
     """Validates what the reference's ``data_ptr<float>()`` calls would and fills pa_params.
 
     ``debug_output``, ``alibi_slopes``, ``softcap`` are accepted and ignored like in the
-    reference (paged_attention_kernel_loop.hpp:175-178,329-342).
+    reference (paged_attention_kernel_loop.hpp:175-178,329-342).  ``int8`` (with ``fp8``, whose
+    scale arguments it shares) selects the integer cache.
     """
     _require(query.is_cuda, "paged attention needs CUDA tensors (no CPU fallback exists)")
     # the reference's data_ptr<float>() calls reject other dtypes (paged_attention_loop.cpp:47-52)
@@ -93,16 +97,16 @@ def build_params(max_logits, exp_sums, tem_output, output, debug_output, query, 
     p.num_blocks = key_cache.size(0)
     p.sm_scale = float(sm_scale)
     p.fp8_scale = float(fp8_scale)
-    p.kv_dtype = _kv_dtype_of(key_cache, fp8)
+    p.kv_dtype = _kv_dtype_of(key_cache, fp8, int8)
     for name, t in (("k_scale_per_head", k_scale_per_head), ("v_scale_per_head", v_scale_per_head)):
         if t is not None:
-            _require(fp8, "per-head scales belong to the FP8 operators")
+            _require(fp8, "per-head scales belong to the FP8 and int8 operators")
             _require(t.dtype == torch.float32 and t.is_contiguous() and t.device == query.device
                      and t.numel() == key_cache.size(2), f"{name} must be float32 [num_kv_heads] on the device")
             setattr(p, name, t.data_ptr())
     for name, t in (("k_scale_per_block", k_scale_per_block), ("v_scale_per_block", v_scale_per_block)):
         if t is not None:
-            _require(fp8, "per-block scales belong to the FP8 operators")
+            _require(fp8, "per-block scales belong to the FP8 and int8 operators")
             _require(t.dtype == torch.float32 and t.is_contiguous() and t.device == query.device
                      and tuple(t.shape) == (key_cache.size(0), key_cache.size(2)),
                      f"{name} must be float32 [num_blocks, num_kv_heads] on the device")

@@ -70,24 +70,30 @@ class AutoDecodePlan:
 
 def paged_attention_auto(plan: AutoDecodePlan, out, query, key_cache, value_cache, block_tables,
                          context_lens, num_queries_per_tokens: int, sm_scale: float,
-                         fp8_scale: float = 1.0, sinks=None) -> None:
+                         fp8_scale: float = 1.0, sinks=None, *, k_scale_per_block=None,
+                         v_scale_per_block=None) -> None:
     """Asynchronous decode attention of a whole batch: loop kernel for the plan's short
     sequences, split-context pair for its long ones.  Both launches work on the caller's
     tensors in place (each is given the list of sequence ids it covers), on two streams that
-    fork from and join the current stream.  `out` [S, H, D] is written for every sequence."""
-    fp8 = key_cache.dtype != torch.float16
+    fork from and join the current stream.  `out` [S, H, D] is written for every sequence.
+    The entry points follow the cache's type (fp16, FP8, int8); `fp8_scale` or the per-block scales
+    are those of an 8-bit cache."""
+    fp8 = key_cache.dtype != torch.float16  # an 8-bit cache
+    int8 = key_cache.dtype == torch.int8
+    prefix = "int8_" if int8 else "fp8_" if fp8 else ""
     dev = plan.device
 
     def launch(sub: _SubBatch, variant: str) -> None:
         p = _shim.build_params(plan.max_logits, plan.exp_sums, plan.tmp_out, out, None, query, key_cache,
                                value_cache, block_tables, context_lens, num_queries_per_tokens, sm_scale,
-                               fp8_scale, key_cache.size(1), sub.max_ctx, plan.alibi, sinks, -1.0, fp8=fp8)
+                               fp8_scale, key_cache.size(1), sub.max_ctx, plan.alibi, sinks, -1.0, fp8=fp8,
+                               int8=int8, k_scale_per_block=k_scale_per_block, v_scale_per_block=v_scale_per_block)
         if variant == "reduce":
             _shim.check_scratch(p, plan.max_logits, plan.exp_sums, plan.tmp_out)
         if sub.count != query.size(0):
             p.num_seqs = sub.count
             p.seq_indices = sub.index.data_ptr()
-        _shim.enqueue_entry(f"launch_kernels_{'fp8_' if fp8 else ''}{variant}", p, dev)
+        _shim.enqueue_entry(f"launch_kernels_{prefix}{variant}", p, dev)
 
     subs = [(sub, variant) for sub, variant in ((plan.loop, "loop"), (plan.reduce, "reduce")) if sub is not None]
     if len(subs) == 1:

@@ -20,7 +20,7 @@
  *
  * Data layouts (reference paged_attention_kernel_loop.hpp:44-62):
  *   query        fp16  [num_seqs, num_heads, head_size]
- *   key_cache    fp16 or 1-byte FP8  [num_blocks, block_size, num_kv_heads, head_size]
+ *   key_cache    fp16, 1-byte FP8 or int8  [num_blocks, block_size, num_kv_heads, head_size]
  *   value_cache  same layout and type as key_cache
  *   block_tables int32 (read as uint32) [num_seqs, max_blocks_per_seq]
  *   context_lens int32 (read as uint32) [num_seqs]
@@ -57,7 +57,8 @@ typedef enum pa_kv_dtype {
   PA_KV_F16 = 0,
   PA_KV_FP8_E5M2 = 1, /* the format the reference bindings hard-wire
                          (paged_attention_fp8_loop/paged_attention_fp8_loop.cpp:43) */
-  PA_KV_FP8_E4M3 = 2  /* e4m3fn bit layout (no infinities, 0x7F/0xFF = NaN) */
+  PA_KV_FP8_E4M3 = 2, /* e4m3fn bit layout (no infinities, 0x7F/0xFF = NaN) */
+  PA_KV_INT8 = 3      /* signed 8-bit integers; value = code * scale (no reference counterpart) */
 } pa_kv_dtype;
 
 typedef struct pa_params {
@@ -88,8 +89,8 @@ typedef struct pa_params {
   uint64_t num_blocks;             /* key_cache.size(0); bounds the TMA descriptor, so a
                                       block id >= num_blocks reads zeros instead of faulting */
   float sm_scale;
-  float fp8_scale; /* per-tensor dequantisation scale of an FP8 cache; ignored for fp16 */
-  int32_t kv_dtype; /* pa_kv_dtype; must match the entry point (fp16 vs FP8) */
+  float fp8_scale; /* per-tensor dequantisation scale of an FP8 or int8 cache; ignored for fp16 */
+  int32_t kv_dtype; /* pa_kv_dtype; must match the entry point (fp16, FP8 or int8) */
   int32_t reserved1;
   /* Optional per-KV-head dequantisation scales of an FP8 cache (device pointers, fp32
    * [num_kv_heads] each, or NULL).  The reference has one scalar fp8_scale
@@ -177,6 +178,14 @@ PA_API int launch_kernels_fp8_loop(const pa_params *p, void *stream, float *us_o
  * (paged_attention_fp8_reduce/launch_kernels_fp8_reduce.h:16-76,78-196). */
 PA_API int launch_kernels_fp8_reduce(const pa_params *p, void *stream, float *us_out);
 
+/* 8-bit integer KV cache (PA_KV_INT8), single pass and split-context; no reference counterpart.
+ * The argument block, the scratch and the two forms are those of the FP8 entry points: a code c
+ * of K dequantises as c * scale with the scale of p->fp8_scale, of its KV head
+ * (k_scale_per_head) or of its block and KV head (k_scale_per_block), V likewise.  A scale of
+ * 0 is a block (or head) of zeros; negative scales are not supported. */
+PA_API int launch_kernels_int8_loop(const pa_params *p, void *stream, float *us_out);
+PA_API int launch_kernels_int8_reduce(const pa_params *p, void *stream, float *us_out);
+
 /* Size in bytes of the scratch array built into the library for
  * launch_kernels_reduce_static_scratch (32 MiB, held by every GPU that loads the library). */
 #define PA_STATIC_SCRATCH_BYTES (32u * 1024u * 1024u)
@@ -228,7 +237,9 @@ typedef enum pa_entry {
   PA_ENTRY_LOOP = 0,
   PA_ENTRY_REDUCE = 1,
   PA_ENTRY_FP8_LOOP = 2,
-  PA_ENTRY_FP8_REDUCE = 3
+  PA_ENTRY_FP8_REDUCE = 3,
+  PA_ENTRY_INT8_LOOP = 4,
+  PA_ENTRY_INT8_REDUCE = 5
 } pa_entry;
 
 /* One decode step with host buffers, in one call (no counterpart in the reference, whose
@@ -351,7 +362,7 @@ PA_API int pa_multi_gpu_gather_out(const pa_device_shard *shards, uint32_t num_s
 typedef struct pa_cache_write_params {
   const void *key;             /* fp16 [num_tokens, num_kv_heads, head_size] */
   const void *value;           /* fp16 [num_tokens, num_kv_heads, head_size] */
-  void *key_cache;             /* [num_blocks, block_size, num_kv_heads, head_size], fp16 or FP8 */
+  void *key_cache;             /* [num_blocks, block_size, num_kv_heads, head_size], fp16, FP8 or int8 */
   void *value_cache;           /* same layout and type as key_cache */
   const int64_t *slot_mapping; /* [num_tokens]: block_id * block_size + row; negative = skip the token */
   uint32_t num_tokens;
@@ -361,7 +372,7 @@ typedef struct pa_cache_write_params {
   uint64_t num_blocks;
   float fp8_scale;             /* stored = x / fp8_scale (the scale the attention entry points take) */
   int32_t kv_dtype;            /* pa_kv_dtype of the cache */
-  /* Optional scales of an FP8 cache that take the place of fp8_scale, the very arrays the
+  /* Optional scales of an 8-bit cache that take the place of fp8_scale, the very arrays the
    * attention entry points take under the same names (pa_params): per KV head, fp32
    * [num_kv_heads], or per block and KV head, fp32 [num_blocks, num_kv_heads].  K and V
    * both or neither, one kind at most; stored = x / scale of the token's head (and block).
@@ -375,7 +386,8 @@ typedef struct pa_cache_write_params {
 /* Appends new K/V tokens to the paged cache in the layout the attention entry points read
  * (reference paged_attention_kernel_loop.hpp:50-51), casting to the cache type: fp16 is
  * copied, FP8 is round-to-nearest-even of x / scale (fp8_scale, or the per-head / per-block
- * scale arrays when given), saturating to the largest finite code.  The reference has no device kernel for this step: its tests fill caches on the host
+ * scale arrays when given), saturating to the largest finite code (int8: to -127 .. 127, NaN
+ * becomes 0).  The reference has no device kernel for this step: its tests fill caches on the host
  * with torch casts (test_paged_fp8cache.py:180-203), which this call reproduces bit for bit for
  * values inside the format's range.  Asynchronous on `stream`. */
 PA_API int pa_reshape_and_cache(const pa_cache_write_params *p, void *stream);

@@ -13,7 +13,7 @@
 
 namespace pa {
 
-enum KvType : int { KV_F16 = 0, KV_E5M2 = 1, KV_E4M3 = 2 };
+enum KvType : int { KV_F16 = 0, KV_E5M2 = 1, KV_E4M3 = 2, KV_I8 = 3 };
 
 struct paged_attention_base_policy {
   static constexpr uint32_t stages = 3;            // reference base policy (:6)

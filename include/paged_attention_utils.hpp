@@ -118,10 +118,19 @@ PA_DEV void mma_m16n8k16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uin
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// ---------------------------------------------------------------- FP8 -> fp16
-// Both formats convert exactly: every finite e5m2 and e4m3 value is representable in fp16.
-// A register holds four FP8 codes (bytes 0..3); results are fp16x2 registers with the first
-// named byte in the low half.
+// -------------------------------------------------------------- 8 bits -> fp16
+// All three formats convert exactly: every finite e5m2 and e4m3 value and every 8-bit integer
+// is representable in fp16.  A register holds four codes (bytes 0..3); results are fp16x2
+// registers with the first named byte in the low half.
+//
+// Integers: the code plus 128 is an unsigned byte u, and the half with the bits 0x6400 | u is
+// 1024 + u, so subtracting 1152 from it leaves the code itself, exactly.  Two byte placements
+// and two packed subtractions for four codes (a cvt per code would run at a quarter of that rate).
+PA_DEV uint32_t int8_biased_to_half2(uint32_t biased) {
+  uint32_t r;
+  asm("sub.f16x2 %0, %1, %2;" : "=r"(r) : "r"(biased), "r"(0x64806480u));
+  return r;
+}
 PA_DEV uint32_t e4m3x2_to_half2(uint16_t pair) {
   uint32_t r;
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(pair));
@@ -131,8 +140,12 @@ PA_DEV uint32_t e4m3x2_to_half2(uint16_t pair) {
 // bytes (0,1) -> lo01, bytes (2,3) -> hi23   (K fragments: consecutive dims per lane)
 template <int KV>
 PA_DEV void fp8x4_to_half2x2(uint32_t v, uint32_t &lo01, uint32_t &hi23) {
-  static_assert(KV == 1 || KV == 2, "FP8 formats only");
-  if constexpr (KV == 1) {
+  static_assert(KV >= 1 && KV <= 3, "8-bit formats only");
+  if constexpr (KV == 3) {
+    const uint32_t u = v ^ 0x80808080u;
+    lo01 = int8_biased_to_half2(__byte_perm(u, 0x64646464u, 0x4140));
+    hi23 = int8_biased_to_half2(__byte_perm(u, 0x64646464u, 0x4342));
+  } else if constexpr (KV == 1) {
     // e5m2 is the high byte of an fp16: move each code into the high byte of a half
     lo01 = __byte_perm(v, 0u, 0x1404);
     hi23 = __byte_perm(v, 0u, 0x3424);
@@ -145,8 +158,12 @@ PA_DEV void fp8x4_to_half2x2(uint32_t v, uint32_t &lo01, uint32_t &hi23) {
 // bytes (0,2) -> even, bytes (1,3) -> odd   (V fragments after a 16-bit transposing load)
 template <int KV>
 PA_DEV void fp8x4_to_even_odd_half2(uint32_t v, uint32_t &even, uint32_t &odd) {
-  static_assert(KV == 1 || KV == 2, "FP8 formats only");
-  if constexpr (KV == 1) {
+  static_assert(KV >= 1 && KV <= 3, "8-bit formats only");
+  if constexpr (KV == 3) {
+    const uint32_t u = v ^ 0x80808080u;
+    even = int8_biased_to_half2(__byte_perm(u, 0x64646464u, 0x4240));
+    odd = int8_biased_to_half2(__byte_perm(u, 0x64646464u, 0x4341));
+  } else if constexpr (KV == 1) {
     even = __byte_perm(v, 0u, 0x2404);
     odd = v & 0xff00ff00u; // bytes 1 and 3 already sit in the high byte of each half
   } else {

@@ -1,0 +1,74 @@
+"""The operators beside the reference's four refuse bad arguments on the host, before any device work."""
+import ctypes
+
+import pytest
+import torch
+
+import flash_attention_factory_b200 as pkg
+from flash_attention_factory_b200 import _cabi
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from flash_attention_factory_b200 import build
+
+    build.build()
+    return pkg.load_library()
+
+
+def _attn(**kw):
+    p = _cabi.PaParams()
+    base = dict(out=0x1000, max_logits=0x2000, exp_sums=0x3000, tmp_out=0x4000, query=0x5000, key_cache=0x6000,
+                value_cache=0x7000, block_tables=0x8000, context_lens=0x9000, num_seqs=2, num_heads=8, head_size=128,
+                num_kv_heads=2, max_num_partitions=1, max_blocks_per_seq=4, block_size=16, num_queries_per_tokens=4,
+                num_blocks=8, sm_scale=0.1, fp8_scale=1.0, kv_dtype=_cabi.KV_INT8)
+    base.update(kw)
+    for k, v in base.items():
+        setattr(p, k, v)
+    return p
+
+
+@pytest.mark.parametrize("entry", ["launch_kernels_int8_loop", "launch_kernels_int8_reduce"])
+def test_int8_entries(lib, entry):
+    def call(**kw):
+        p = _attn(**kw)
+        return getattr(lib, entry)(ctypes.byref(p), None, None), lib.pa_last_error().decode()
+
+    for kv in (_cabi.KV_F16, _cabi.KV_FP8_E5M2, _cabi.KV_FP8_E4M3, 4, -1):
+        rc, msg = call(kv_dtype=kv)
+        assert rc == _cabi.PA_ERR_BAD_ARG and "kv_dtype" in msg
+    assert call(head_size=96)[0] == _cabi.PA_ERR_UNSUPPORTED
+    assert call(fp8_scale=0.0)[0] == _cabi.PA_ERR_BAD_ARG
+    assert call(query=0)[0] == _cabi.PA_ERR_BAD_ARG
+    assert "together" in call(k_scale_per_block=0x1000)[1]
+    assert "exclude" in call(k_scale_per_block=0x1000, v_scale_per_block=0x1000, k_scale_per_head=0x1000)[1]
+    assert call(num_seqs=0)[0] == _cabi.PA_OK
+    assert getattr(lib, entry)(None, None, None) == _cabi.PA_ERR_BAD_ARG
+
+
+def test_fp8_entries_refuse_an_int8_cache(lib):
+    for entry in ("launch_kernels_loop", "launch_kernels_reduce", "launch_kernels_fp8_loop", "launch_kernels_fp8_reduce"):
+        assert getattr(lib, entry)(ctypes.byref(_attn()), None, None) == _cabi.PA_ERR_BAD_ARG
+
+
+def test_int8_modules_mirror_the_fp8_surface():
+    import inspect
+
+    from flash_attention_factory_b200 import lib as shim
+
+    for variant in ("loop", "reduce"):
+        for fn in ("run", "params", "enqueue"):
+            a = inspect.signature(getattr(getattr(shim, f"paged_attention_int8_{variant}"), fn))
+            b = inspect.signature(getattr(getattr(shim, f"paged_attention_fp8_{variant}"), fn))
+            assert [n.replace("int8_scale", "fp8_scale") for n in a.parameters] == list(b.parameters)
+
+
+def test_int8_modules_refuse_cpu_tensors():
+    from flash_attention_factory_b200 import lib as shim
+
+    c = torch.zeros(1, 16, 1, 128, dtype=torch.int8)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        shim.paged_attention_int8_loop.run(torch.zeros(1, 2, 1), torch.zeros(1, 2, 1), torch.zeros(1, 2, 1, 128).half(),
+                                           torch.zeros(1, 2, 128).half(), torch.zeros(1), torch.zeros(1, 2, 128).half(), c, c,
+                                           torch.zeros(1, 1, dtype=torch.int32), torch.ones(1, dtype=torch.int32), 2, 0.1,
+                                           1.0, 16, 1, torch.ones(2), None, -1.0)
