@@ -34,6 +34,7 @@ EXPORTED_SYMBOLS = (
     "launch_kernels_int8_reduce",
     "launch_kernels_reduce_static_scratch",
     "pa_reshape_and_cache",
+    "pa_rope_and_cache",
     "pa_query_policy",
     "pa_partition_size",
     "pa_last_error",
@@ -127,6 +128,26 @@ class PaCacheWriteParams(ctypes.Structure):
         ("v_scale_per_head", ctypes.c_void_p),
         ("k_scale_per_block", ctypes.c_void_p),
         ("v_scale_per_block", ctypes.c_void_p),
+    ]
+
+
+class PaRopeCacheParams(ctypes.Structure):
+    """struct pa_rope_cache_params of include/paged_attention_b200.h."""
+
+    _fields_ = [
+        ("cache", PaCacheWriteParams),
+        ("query", ctypes.c_void_p),
+        ("query_out", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("cos_sin", ctypes.c_void_p),
+        ("max_position", ctypes.c_uint64),
+        ("rotary_dim", ctypes.c_uint32),
+        ("num_heads", ctypes.c_uint32),
+        ("query_token_stride", ctypes.c_uint64),
+        ("key_token_stride", ctypes.c_uint64),
+        ("value_token_stride", ctypes.c_uint64),
+        ("interleaved", ctypes.c_uint32),
+        ("reserved", ctypes.c_uint32),
     ]
 
 
@@ -225,6 +246,8 @@ def load_library() -> ctypes.CDLL:
     lib.launch_kernels_reduce_static_scratch.restype = ctypes.c_int
     lib.pa_reshape_and_cache.argtypes = [ctypes.POINTER(PaCacheWriteParams), ctypes.c_void_p]
     lib.pa_reshape_and_cache.restype = ctypes.c_int
+    lib.pa_rope_and_cache.argtypes = [ctypes.POINTER(PaRopeCacheParams), ctypes.c_void_p]
+    lib.pa_rope_and_cache.restype = ctypes.c_int
     lib.pa_query_policy.argtypes = [ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32,
                                     ctypes.POINTER(PaPolicyInfo)]
     lib.pa_query_policy.restype = ctypes.c_int

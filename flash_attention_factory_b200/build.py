@@ -36,6 +36,7 @@ SOURCES = [
     "launch_kernels_int8_loop.cu",
     "launch_kernels_int8_reduce.cu",
     "cache_write.cu",
+    "rope_cache.cu",
 ]
 # the aid library links its own copy of the shared host pieces and nothing of the product
 AIDS_SOURCES = ["host_common.cu", "test_aids.cu"]

@@ -4,6 +4,9 @@
 ([num_blocks, block_size, num_kv_heads, head_size]) and casts them to the cache type on the
 way.  The reference builds its caches on the host with torch casts
 (test_paged_fp8cache.py:180-203); this is the device-side counterpart of that fixture code.
+
+`rope_and_cache` does the same with the rotary position embedding applied to K, and to the
+step's queries, in the same launch.
 """
 from __future__ import annotations
 
@@ -24,6 +27,20 @@ def _kv_dtype(cache: torch.Tensor) -> int:
     if cache.dtype == torch.int8:
         return _cabi.KV_INT8
     raise RuntimeError(f"unsupported cache dtype {cache.dtype}")
+
+
+def _set_scales(p, key, key_cache, k_scale_per_head, v_scale_per_head, k_scale_per_block, v_scale_per_block) -> None:
+    per_head, per_block = (key.size(1),), (key_cache.size(0), key.size(1))
+    for name, t, shape in (("k_scale_per_head", k_scale_per_head, per_head),
+                           ("v_scale_per_head", v_scale_per_head, per_head),
+                           ("k_scale_per_block", k_scale_per_block, per_block),
+                           ("v_scale_per_block", v_scale_per_block, per_block)):
+        if t is None:
+            continue
+        if (t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous()
+                or t.device != key.device):
+            raise RuntimeError(f"{name} must be a contiguous float32 tensor of shape {shape} on the cache's device")
+        setattr(p, name, t.data_ptr())
 
 
 def reshape_and_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor,
@@ -59,18 +76,101 @@ def reshape_and_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.T
     p.block_size, p.num_blocks = key_cache.size(1), key_cache.size(0)
     p.fp8_scale = float(fp8_scale)
     p.kv_dtype = _kv_dtype(key_cache)
-    per_head, per_block = (key.size(1),), (key_cache.size(0), key.size(1))
-    for name, t, shape in (("k_scale_per_head", k_scale_per_head, per_head),
-                           ("v_scale_per_head", v_scale_per_head, per_head),
-                           ("k_scale_per_block", k_scale_per_block, per_block),
-                           ("v_scale_per_block", v_scale_per_block, per_block)):
-        if t is None:
-            continue
-        if (t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous()
-                or t.device != key.device):
-            raise RuntimeError(f"{name} must be a contiguous float32 tensor of shape {shape} on the cache's device")
-        setattr(p, name, t.data_ptr())
+    _set_scales(p, key, key_cache, k_scale_per_head, v_scale_per_head, k_scale_per_block, v_scale_per_block)
     lib = _cabi.load_library()
     with torch.cuda.device(key.device):
         stream = torch.cuda.current_stream(key.device).cuda_stream
         _cabi.check(lib.pa_reshape_and_cache(ctypes.byref(p), ctypes.c_void_p(stream)))
+
+
+def _require(cond: bool, msg: str) -> None:
+    if not cond:
+        raise RuntimeError(msg)
+
+
+def _token_rows(t: torch.Tensor, name: str, device) -> int:
+    """Checks fp16 rows [T, heads, D] whose tokens may lie any stride apart (slices of one projection's
+    output); returns that stride in elements."""
+    _require(t.is_cuda and t.device == device and t.dtype == torch.float16 and t.dim() == 3,
+             f"{name} must be a float16 tensor [tokens, heads, head_size] on the cache's device")
+    _require(t.stride(2) == 1 and (t.size(1) == 1 or t.stride(1) == t.size(2)),
+             f"the heads of a token of {name} must be contiguous")
+    stride = t.stride(0) if t.size(0) > 1 else t.size(1) * t.size(2)
+    _require(stride >= 0 and stride % 8 == 0, f"the token stride of {name} must be a multiple of 8 elements")
+    return stride
+
+
+def _check_caches(key, value, key_cache, value_cache) -> None:
+    _require(key_cache.is_cuda and key_cache.is_contiguous() and value_cache.is_contiguous()
+             and value_cache.device == key_cache.device, "the caches must be contiguous CUDA tensors on one device "
+             "(no CPU fallback exists)")
+    _require(key_cache.dim() == 4 and key_cache.shape == value_cache.shape and key_cache.dtype == value_cache.dtype,
+             "key_cache and value_cache must match")
+    _require(key.shape == value.shape and tuple(key_cache.shape[2:]) == tuple(key.shape[1:]),
+             "cache must be [num_blocks, block_size, num_kv_heads, head_size]")
+
+
+def _check_rotation(cos_sin, device) -> None:
+    _require(cos_sin.dtype == torch.float32 and cos_sin.dim() == 2 and cos_sin.is_contiguous() and cos_sin.device == device,
+             "cos_sin must be a contiguous float32 tensor [max_position, rotary_dim] on the cache's device")
+
+
+def _check_queries(p, query, query_out, key) -> None:
+    """Fills the query part of an argument block."""
+    _require((query is None) == (query_out is None), "query and query_out must be given together")
+    if query is None:
+        return
+    p.query_token_stride = _token_rows(query, "query", key.device)
+    _require(query.size(0) == key.size(0) and query.size(2) == key.size(2), "query and key must have the same tokens and head_size")
+    _require(query_out.shape == query.shape and query_out.dtype == torch.float16 and query_out.is_contiguous()
+             and query_out.device == key.device, "query_out must be a contiguous float16 tensor of query's shape")
+    p.num_heads, p.query, p.query_out = query.size(1), query.data_ptr(), query_out.data_ptr()
+
+
+def _call(fn, p, device) -> None:
+    """Runs a writer on torch's current stream of `device`, with that device current."""
+    if torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device):
+            return _call(fn, p, torch.device("cuda", torch.cuda.current_device()))
+    _cabi.check(fn(ctypes.byref(p), ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)))
+
+
+def rope_and_cache(query, key: torch.Tensor, value: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor,
+                   query_out, key_cache: torch.Tensor, value_cache: torch.Tensor, slot_mapping: torch.Tensor,
+                   fp8_scale: float = 1.0, *, interleaved: bool = False, k_scale_per_head=None, v_scale_per_head=None,
+                   k_scale_per_block=None, v_scale_per_block=None) -> None:
+    """`reshape_and_cache` with the rotary position embedding applied to K and to the step's queries.
+
+    query fp16 [T, H, D] and key / value fp16 [T, HK, D] may be slices of one projection's output (the
+    heads of a token contiguous, tokens any multiple of 8 elements apart); query and query_out
+    (contiguous, or query itself if that is contiguous) may both be None.  positions int64 [T];
+    cos_sin float32 [max_position, R]: R / 2 cosines, then the sines, of a position's angles; the first R
+    dims of a head (a multiple of 16) are rotated, as pairs (i, i + R / 2), or (2 i, 2 i + 1) with
+    `interleaved`.  The rotation runs in fp32 and is rounded once, to fp16 or to the cache's code.
+
+    Slots, cache types and scales are those of `reshape_and_cache`.  A token with a negative slot (padding),
+    or whose slot or position is out of range, is skipped: its cache and query_out rows stay as they
+    were.  Asynchronous on torch's current stream.
+    """
+    _check_caches(key, value, key_cache, value_cache)
+    device = key_cache.device
+    p = _cabi.PaRopeCacheParams()
+    p.key_token_stride = _token_rows(key, "key", device)
+    p.value_token_stride = _token_rows(value, "value", device)
+    t = key.size(0)
+    for name, x in (("slot_mapping", slot_mapping), ("positions", positions)):
+        _require(x.dtype == torch.int64 and x.numel() == t and x.is_contiguous() and x.device == device,
+                 f"{name} must be int64 with one entry per token on the cache's device")
+    _check_rotation(cos_sin, device)
+    _check_queries(p, query, query_out, key)
+    c = p.cache
+    c.key, c.value = key.data_ptr(), value.data_ptr()
+    c.key_cache, c.value_cache = key_cache.data_ptr(), value_cache.data_ptr()
+    c.slot_mapping = slot_mapping.data_ptr()
+    c.num_tokens, c.num_kv_heads, c.head_size = t, key.size(1), key.size(2)
+    c.block_size, c.num_blocks = key_cache.size(1), key_cache.size(0)
+    c.fp8_scale, c.kv_dtype = float(fp8_scale), _kv_dtype(key_cache)
+    _set_scales(c, key, key_cache, k_scale_per_head, v_scale_per_head, k_scale_per_block, v_scale_per_block)
+    p.positions, p.cos_sin = positions.data_ptr(), cos_sin.data_ptr()
+    p.max_position, p.rotary_dim, p.interleaved = cos_sin.size(0), cos_sin.size(1), int(interleaved)
+    _call(_cabi.load_library().pa_rope_and_cache, p, device)

@@ -9,11 +9,9 @@
 // itself for an fp16 cache.  The scale is fp8_scale, or the
 // entry of the token's KV head (and block) in the per-head / per-block scale arrays that the
 // attention entry points read back under the same names.
-#include <cuda_fp16.h>
-#include <cuda_fp8.h>
-
 #include <cmath>
 
+#include "cache_codes.cuh"
 #include "launch_common.cuh"
 
 namespace pa {
@@ -21,12 +19,6 @@ namespace pa {
 // 8 fp16 values (one 16-byte load) -> 8 cache elements
 // `exact_rcp` != 0 means 1 / scale is a power of two, so multiplying by it is exact and
 // equals the division bit for bit; otherwise an IEEE division keeps the torch arithmetic.
-// One value over its scale -> the nearest integer of -127 .. 127 (ties to even; NaN -> 0).  -128 stays
-// unused so that the codes are symmetric.
-__device__ __forceinline__ uint32_t int8_code(float x) {
-  return static_cast<uint32_t>(max(-127, min(127, __float2int_rn(x)))) & 0xffu;
-}
-
 template <int KV>
 __device__ __forceinline__ void store_converted(void *dst_row, uint32_t elem, uint4 v, float scale,
                                                 float exact_rcp) {
@@ -41,27 +33,17 @@ __device__ __forceinline__ void store_converted(void *dst_row, uint32_t elem, ui
       // (x.float() / scale).to(float8) for every value inside the format's range
       float2 a = __half22float2(h[2 * i]);
       float2 b = __half22float2(h[2 * i + 1]);
-      constexpr __nv_fp8_interpretation_t fmt = (KV == KV_E5M2) ? __NV_E5M2 : __NV_E4M3;
       if (exact_rcp != 0.f) {
         a.x *= exact_rcp; a.y *= exact_rcp; b.x *= exact_rcp; b.y *= exact_rcp;
       } else {
         a.x = __fdiv_rn(a.x, scale); a.y = __fdiv_rn(a.y, scale);
         b.x = __fdiv_rn(b.x, scale); b.y = __fdiv_rn(b.y, scale);
       }
-      if constexpr (KV == KV_I8) {
-        packed[i] = int8_code(a.x) | (int8_code(a.y) << 8) | (int8_code(b.x) << 16) | (int8_code(b.y) << 24);
-      } else {
-        const uint32_t lo = __nv_cvt_float2_to_fp8x2(a, __NV_SATFINITE, fmt);
-        const uint32_t hi = __nv_cvt_float2_to_fp8x2(b, __NV_SATFINITE, fmt);
-        packed[i] = lo | (hi << 16);
-      }
+      packed[i] = pack_codes<KV>(a.x, a.y, b.x, b.y);
     }
     *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(dst_row) + elem) = make_uint2(packed[0], packed[1]);
   }
 }
-
-// Where the scale of an element comes from.
-enum ScaleKind : int { SCALE_SCALAR = 0, SCALE_PER_HEAD = 1, SCALE_PER_BLOCK = 2 };
 
 struct ScaleArrays {
   const float *k; // [num_kv_heads] or [num_blocks, num_kv_heads]; unused for SCALE_SCALAR
@@ -118,32 +100,11 @@ reshape_and_cache_kernel(const __half *__restrict__ key, const __half *__restric
 
 extern "C" PA_API int pa_reshape_and_cache(const pa_cache_write_params *p, void *stream) {
   using namespace pa;
-  if (p == nullptr) return fail(PA_ERR_BAD_ARG, "params is null");
-  if (p->kv_dtype != PA_KV_F16 && p->kv_dtype != PA_KV_FP8_E5M2 && p->kv_dtype != PA_KV_FP8_E4M3 &&
-      p->kv_dtype != PA_KV_INT8)
-    return fail(PA_ERR_BAD_ARG, "unknown kv_dtype %d", p->kv_dtype);
+  if (int rc = validate_cache_write(p)) return rc;
   if (p->num_tokens == 0) return PA_OK;
-  if (!p->key || !p->value || !p->key_cache || !p->value_cache || !p->slot_mapping)
-    return fail(PA_ERR_BAD_ARG, "a required pointer is null");
+  const bool per_head = p->k_scale_per_head != nullptr;
+  const bool per_block = p->k_scale_per_block != nullptr;
   const uint64_t row_elems = static_cast<uint64_t>(p->num_kv_heads) * p->head_size;
-  if (row_elems == 0 || row_elems % 8 != 0 || row_elems > (1u << 20))
-    return fail(PA_ERR_BAD_ARG, "num_kv_heads * head_size must be a positive multiple of 8");
-  if (p->block_size == 0 || p->num_blocks == 0) return fail(PA_ERR_BAD_ARG, "empty cache");
-  const bool per_head = p->k_scale_per_head != nullptr || p->v_scale_per_head != nullptr;
-  const bool per_block = p->k_scale_per_block != nullptr || p->v_scale_per_block != nullptr;
-  if (per_head && (p->k_scale_per_head == nullptr || p->v_scale_per_head == nullptr))
-    return fail(PA_ERR_BAD_ARG, "k_scale_per_head and v_scale_per_head must be given together");
-  if (per_block && (p->k_scale_per_block == nullptr || p->v_scale_per_block == nullptr))
-    return fail(PA_ERR_BAD_ARG, "k_scale_per_block and v_scale_per_block must be given together");
-  if (per_head && per_block) return fail(PA_ERR_BAD_ARG, "per-head and per-block scales exclude each other");
-  if ((per_head || per_block) && p->kv_dtype == PA_KV_F16)
-    return fail(PA_ERR_BAD_ARG, "scale arrays need an FP8 or int8 cache");
-  if ((per_head || per_block) && (p->head_size == 0 || p->head_size % 8 != 0))
-    return fail(PA_ERR_BAD_ARG, "scale arrays need a head_size that is a multiple of 8");
-  if (p->kv_dtype != PA_KV_F16 && !per_head && !per_block && !(p->fp8_scale > 0.f))
-    return fail(PA_ERR_BAD_ARG, "fp8_scale must be positive and finite");
-  if (!aligned16(p->key) || !aligned16(p->value) || !aligned16(p->key_cache) || !aligned16(p->value_cache))
-    return fail(PA_ERR_BAD_ARG, "key / value / caches must be 16-byte aligned");
   const uint64_t num_slots = p->num_blocks * p->block_size;
   // a power-of-two scale (1.0 included) has an exact reciprocal: no division needed
   float exact_rcp = 0.f;

@@ -169,6 +169,59 @@ inline int validate_params(const pa_params *p, bool fp8_entry, bool needs_scratc
   return PA_OK;
 }
 
+// Checks of the cache writers that take a slot per token.
+inline int validate_cache_write(const pa_cache_write_params *p) {
+  if (p == nullptr) return fail(PA_ERR_BAD_ARG, "params is null");
+  if (p->kv_dtype != PA_KV_F16 && p->kv_dtype != PA_KV_FP8_E5M2 && p->kv_dtype != PA_KV_FP8_E4M3 &&
+      p->kv_dtype != PA_KV_INT8)
+    return fail(PA_ERR_BAD_ARG, "unknown kv_dtype %d", p->kv_dtype);
+  if (p->num_tokens == 0) return PA_OK; // nothing to do; the writer returns early
+  if (!p->key || !p->value || !p->key_cache || !p->value_cache || !p->slot_mapping)
+    return fail(PA_ERR_BAD_ARG, "a required pointer is null");
+  const uint64_t row_elems = static_cast<uint64_t>(p->num_kv_heads) * p->head_size;
+  if (row_elems == 0 || row_elems % 8 != 0 || row_elems > (1u << 20))
+    return fail(PA_ERR_BAD_ARG, "num_kv_heads * head_size must be a positive multiple of 8");
+  if (p->block_size == 0 || p->num_blocks == 0) return fail(PA_ERR_BAD_ARG, "empty cache");
+  const bool per_head = p->k_scale_per_head != nullptr || p->v_scale_per_head != nullptr;
+  const bool per_block = p->k_scale_per_block != nullptr || p->v_scale_per_block != nullptr;
+  if (per_head && (p->k_scale_per_head == nullptr || p->v_scale_per_head == nullptr))
+    return fail(PA_ERR_BAD_ARG, "k_scale_per_head and v_scale_per_head must be given together");
+  if (per_block && (p->k_scale_per_block == nullptr || p->v_scale_per_block == nullptr))
+    return fail(PA_ERR_BAD_ARG, "k_scale_per_block and v_scale_per_block must be given together");
+  if (per_head && per_block) return fail(PA_ERR_BAD_ARG, "per-head and per-block scales exclude each other");
+  if ((per_head || per_block) && p->kv_dtype == PA_KV_F16)
+    return fail(PA_ERR_BAD_ARG, "scale arrays need an FP8 or int8 cache");
+  if ((per_head || per_block) && (p->head_size == 0 || p->head_size % 8 != 0))
+    return fail(PA_ERR_BAD_ARG, "scale arrays need a head_size that is a multiple of 8");
+  if (p->kv_dtype != PA_KV_F16 && !per_head && !per_block && !(p->fp8_scale > 0.f))
+    return fail(PA_ERR_BAD_ARG, "fp8_scale must be positive and finite");
+  if (!aligned16(p->key) || !aligned16(p->value) || !aligned16(p->key_cache) || !aligned16(p->value_cache))
+    return fail(PA_ERR_BAD_ARG, "key / value / caches must be 16-byte aligned");
+  return PA_OK;
+}
+
+// Checks of the writers that rotate: head and rotation sizes, the queries, the token strides.
+inline int validate_rotation(uint32_t head_size, uint32_t rotary_dim, const float *cos_sin, uint64_t max_position,
+                             uint32_t num_heads, const void *query, const void *query_out, uint64_t query_stride,
+                             uint64_t key_stride, uint64_t value_stride) {
+  if (head_size == 0 || head_size % 16 != 0 || head_size > 512)
+    return fail(PA_ERR_UNSUPPORTED, "head_size must be a multiple of 16, at most 512");
+  if (cos_sin != nullptr) {
+    if (rotary_dim == 0 || rotary_dim % 16 != 0 || rotary_dim > head_size)
+      return fail(PA_ERR_UNSUPPORTED, "rotary_dim must be a positive multiple of 16, at most head_size");
+    if (max_position == 0) return fail(PA_ERR_BAD_ARG, "the rotation table is empty");
+    if (!aligned16(cos_sin)) return fail(PA_ERR_BAD_ARG, "cos_sin must be 16-byte aligned");
+  }
+  if ((query == nullptr) != (query_out == nullptr))
+    return fail(PA_ERR_BAD_ARG, "query and query_out must be given together");
+  if (query != nullptr && (num_heads == 0 || num_heads > 65535u))
+    return fail(PA_ERR_BAD_ARG, "num_heads must be in 1..65535 where queries are given");
+  if (!aligned16(query) || !aligned16(query_out)) return fail(PA_ERR_BAD_ARG, "query / query_out must be 16-byte aligned");
+  if (query_stride % 8 != 0 || key_stride % 8 != 0 || value_stride % 8 != 0)
+    return fail(PA_ERR_BAD_ARG, "token strides must be multiples of 8 elements");
+  return PA_OK;
+}
+
 // ------------------------------------------------------------------ geometry
 struct DeviceInfo {
   int sm_count;

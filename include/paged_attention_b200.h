@@ -392,6 +392,35 @@ typedef struct pa_cache_write_params {
  * values inside the format's range.  Asynchronous on `stream`. */
 PA_API int pa_reshape_and_cache(const pa_cache_write_params *p, void *stream);
 
+/* Arguments of pa_rope_and_cache. */
+typedef struct pa_rope_cache_params {
+  /* The cache side, as for pa_reshape_and_cache, but the rows of key and value
+   * ([num_kv_heads, head_size] fp16) lie key_token_stride / value_token_stride elements apart. */
+  pa_cache_write_params cache;
+  const void *query;        /* fp16 rows of [num_heads, head_size], or NULL: no queries */
+  void *query_out;          /* fp16 [num_tokens, num_heads, head_size], contiguous; may be query itself
+                               if that is contiguous */
+  const int64_t *positions; /* [num_tokens] */
+  const float *cos_sin;     /* fp32 [max_position, rotary_dim]: rotary_dim / 2 cosines, then the sines */
+  uint64_t max_position;
+  uint32_t rotary_dim;      /* leading dims of a head that are rotated: a multiple of 16, <= head_size */
+  uint32_t num_heads;       /* query heads; 0 without queries */
+  uint64_t query_token_stride; /* elements between two tokens' rows; multiples of 8 */
+  uint64_t key_token_stride;
+  uint64_t value_token_stride;
+  uint32_t interleaved;     /* pairs (2 i, 2 i + 1) instead of (i, i + rotary_dim / 2) */
+  uint32_t reserved;
+} pa_rope_cache_params;
+
+/* Appends new K/V tokens to the paged cache with the rotary position embedding applied to K (and to
+ * the step's queries) on the way (no reference counterpart).  With c, s the cosine and sine of row
+ * positions[t] of cos_sin for pair i: a' = a c - b s, b' = b c + a s in fp32, one rounding to fp16
+ * (query_out, fp16 caches) or to the cache's 8-bit code; V and the dims behind rotary_dim pass through.
+ * Formats, scales and slots are those of pa_reshape_and_cache.  A token whose slot is negative or
+ * outside the cache, or whose position is outside the table, is skipped altogether: its cache and
+ * query_out rows stay as they were.  Slots of one call have to differ.  head_size: a multiple of 16. */
+PA_API int pa_rope_and_cache(const pa_rope_cache_params *p, void *stream);
+
 /* Compile-time policy of include/paged_attention_policy_v2.hpp as data
  * (reference include/paged_attention_policy_v2.hpp:5-100).  Returns
  * PA_ERR_UNSUPPORTED for triples the launchers reject. */

@@ -72,3 +72,53 @@ def test_int8_modules_refuse_cpu_tensors():
                                            torch.zeros(1, 2, 128).half(), torch.zeros(1), torch.zeros(1, 2, 128).half(), c, c,
                                            torch.zeros(1, 1, dtype=torch.int32), torch.ones(1, dtype=torch.int32), 2, 0.1,
                                            1.0, 16, 1, torch.ones(2), None, -1.0)
+
+
+def _cache_write(p, **kw):
+    base = dict(key=0x1000, value=0x2000, key_cache=0x3000, value_cache=0x4000, slot_mapping=0x5000, num_tokens=3,
+                num_kv_heads=2, head_size=128, block_size=16, num_blocks=4, fp8_scale=1.0, kv_dtype=_cabi.KV_INT8)
+    base.update(kw)
+    for k, v in base.items():
+        setattr(p, k, v)
+
+
+def test_rope_and_cache(lib):
+    def call(cache=None, **kw):
+        p = _cabi.PaRopeCacheParams()
+        _cache_write(p.cache, **(cache or {}))
+        base = dict(query=0x6000, query_out=0x7000, positions=0x8000, cos_sin=0x9000, max_position=64, rotary_dim=128,
+                    num_heads=4, query_token_stride=512, key_token_stride=256, value_token_stride=256)
+        base.update(kw)
+        for k, v in base.items():
+            setattr(p, k, v)
+        return lib.pa_rope_and_cache(ctypes.byref(p), None), lib.pa_last_error().decode()
+
+    bad, unsupported = _cabi.PA_ERR_BAD_ARG, _cabi.PA_ERR_UNSUPPORTED
+    assert lib.pa_rope_and_cache(None, None) == bad
+    assert call(cache=dict(num_tokens=0))[0] == _cabi.PA_OK
+    assert call(cache=dict(kv_dtype=9))[0] == bad
+    assert call(cache=dict(key=0x1008))[0] == bad
+    assert call(cache=dict(fp8_scale=0.0))[0] == bad
+    assert call(cache=dict(head_size=72))[0] == unsupported
+    assert call(cache=dict(head_size=528))[0] == unsupported
+    for r in (0, 8, 24, 144):
+        assert call(rotary_dim=r)[0] == unsupported
+    assert call(max_position=0)[0] == bad
+    assert call(positions=0)[0] == bad
+    assert call(cos_sin=0)[0] == bad
+    assert call(cos_sin=0x9004)[0] == bad
+    assert "together" in call(query=0)[1]
+    assert "together" in call(query_out=0)[1]
+    assert call(num_heads=0)[0] == bad
+    assert call(query=0x6004)[0] == bad
+    assert call(key_token_stride=260)[0] == bad
+
+
+def test_cache_ops_refuse_cpu_tensors_and_odd_layouts():
+    from flash_attention_factory_b200 import cache_ops
+
+    k = torch.zeros(2, 1, 64).half()
+    kc = torch.zeros(1, 16, 1, 64, dtype=torch.int8)
+    i = torch.zeros(2, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        cache_ops.rope_and_cache(None, k, k, i, torch.zeros(4, 64), None, kc, kc, i)
