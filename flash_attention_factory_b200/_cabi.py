@@ -32,9 +32,12 @@ EXPORTED_SYMBOLS = (
     "launch_kernels_fp8_reduce",
     "launch_kernels_int8_loop",
     "launch_kernels_int8_reduce",
+    "launch_kernels_diff",
+    "pa_diff_num_partitions",
     "launch_kernels_reduce_static_scratch",
     "pa_reshape_and_cache",
     "pa_rope_and_cache",
+    "pa_append_block_scaled",
     "pa_query_policy",
     "pa_partition_size",
     "pa_last_error",
@@ -88,6 +91,18 @@ class PaParams(ctypes.Structure):
         ("block_table_offsets", ctypes.c_void_p),
         ("k_scale_per_block", ctypes.c_void_p),
         ("v_scale_per_block", ctypes.c_void_p),
+    ]
+
+
+class PaDiffParams(ctypes.Structure):
+    """struct pa_diff_params of include/paged_attention_b200.h."""
+
+    _fields_ = [
+        ("attn", PaParams),
+        ("lambdas", ctypes.c_void_p),
+        ("norm_weight", ctypes.c_void_p),
+        ("norm_eps", ctypes.c_float),
+        ("norm_scale", ctypes.c_float),
     ]
 
 
@@ -148,6 +163,40 @@ class PaRopeCacheParams(ctypes.Structure):
         ("value_token_stride", ctypes.c_uint64),
         ("interleaved", ctypes.c_uint32),
         ("reserved", ctypes.c_uint32),
+    ]
+
+
+class PaBlockScaledParams(ctypes.Structure):
+    """struct pa_block_scaled_params of include/paged_attention_b200.h."""
+
+    _fields_ = [
+        ("key", ctypes.c_void_p),
+        ("value", ctypes.c_void_p),
+        ("key_cache", ctypes.c_void_p),
+        ("value_cache", ctypes.c_void_p),
+        ("k_scale_per_block", ctypes.c_void_p),
+        ("v_scale_per_block", ctypes.c_void_p),
+        ("block_tables", ctypes.c_void_p),
+        ("context_lens", ctypes.c_void_p),
+        ("cu_tokens", ctypes.c_void_p),
+        ("num_seqs", ctypes.c_uint32),
+        ("num_tokens", ctypes.c_uint32),
+        ("num_kv_heads", ctypes.c_uint32),
+        ("head_size", ctypes.c_uint32),
+        ("block_size", ctypes.c_uint32),
+        ("max_blocks_per_seq", ctypes.c_uint32),
+        ("num_blocks", ctypes.c_uint64),
+        ("kv_dtype", ctypes.c_int32),
+        ("interleaved", ctypes.c_uint32),
+        ("cos_sin", ctypes.c_void_p),
+        ("max_position", ctypes.c_uint64),
+        ("rotary_dim", ctypes.c_uint32),
+        ("num_heads", ctypes.c_uint32),
+        ("query", ctypes.c_void_p),
+        ("query_out", ctypes.c_void_p),
+        ("query_token_stride", ctypes.c_uint64),
+        ("key_token_stride", ctypes.c_uint64),
+        ("value_token_stride", ctypes.c_uint64),
     ]
 
 
@@ -242,12 +291,18 @@ def load_library() -> ctypes.CDLL:
         fn = getattr(lib, name)
         fn.argtypes = launcher_args
         fn.restype = ctypes.c_int
+    lib.launch_kernels_diff.argtypes = [ctypes.POINTER(PaDiffParams), ctypes.c_void_p, ctypes.POINTER(ctypes.c_float)]
+    lib.launch_kernels_diff.restype = ctypes.c_int
+    lib.pa_diff_num_partitions.argtypes = [ctypes.c_uint32] * 4
+    lib.pa_diff_num_partitions.restype = ctypes.c_uint32
     lib.launch_kernels_reduce_static_scratch.argtypes = [ctypes.POINTER(PaParams), ctypes.c_void_p]
     lib.launch_kernels_reduce_static_scratch.restype = ctypes.c_int
     lib.pa_reshape_and_cache.argtypes = [ctypes.POINTER(PaCacheWriteParams), ctypes.c_void_p]
     lib.pa_reshape_and_cache.restype = ctypes.c_int
     lib.pa_rope_and_cache.argtypes = [ctypes.POINTER(PaRopeCacheParams), ctypes.c_void_p]
     lib.pa_rope_and_cache.restype = ctypes.c_int
+    lib.pa_append_block_scaled.argtypes = [ctypes.POINTER(PaBlockScaledParams), ctypes.c_void_p]
+    lib.pa_append_block_scaled.restype = ctypes.c_int
     lib.pa_query_policy.argtypes = [ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32,
                                     ctypes.POINTER(PaPolicyInfo)]
     lib.pa_query_policy.restype = ctypes.c_int

@@ -35,8 +35,12 @@ SOURCES = [
     "launch_kernels_fp8_reduce.cu",
     "launch_kernels_int8_loop.cu",
     "launch_kernels_int8_reduce.cu",
+    "launch_kernels_diff.cu",
+    "launch_kernels_diff_fp8.cu",
+    "launch_kernels_diff_int8.cu",
     "cache_write.cu",
     "rope_cache.cu",
+    "block_scaled_append.cu",
 ]
 # the aid library links its own copy of the shared host pieces and nothing of the product
 AIDS_SOURCES = ["host_common.cu", "test_aids.cu"]

@@ -6,7 +6,8 @@ way.  The reference builds its caches on the host with torch casts
 (test_paged_fp8cache.py:180-203); this is the device-side counterpart of that fixture code.
 
 `rope_and_cache` does the same with the rotary position embedding applied to K, and to the
-step's queries, in the same launch.
+step's queries, in the same launch.  `append_block_scaled` appends to an 8-bit cache that keeps a scale
+for each block of tokens and KV head, and keeps those scales.
 """
 from __future__ import annotations
 
@@ -174,3 +175,54 @@ def rope_and_cache(query, key: torch.Tensor, value: torch.Tensor, positions: tor
     p.positions, p.cos_sin = positions.data_ptr(), cos_sin.data_ptr()
     p.max_position, p.rotary_dim, p.interleaved = cos_sin.size(0), cos_sin.size(1), int(interleaved)
     _call(_cabi.load_library().pa_rope_and_cache, p, device)
+
+
+def append_block_scaled(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                        k_scale_per_block: torch.Tensor, v_scale_per_block: torch.Tensor, block_tables: torch.Tensor,
+                        context_lens: torch.Tensor, *, cu_tokens=None, query=None, query_out=None, cos_sin=None,
+                        interleaved: bool = False) -> None:
+    """Appends new tokens to an int8 or FP8 cache with one scale per block of tokens and KV head.
+
+    Sequence i's new tokens are rows cu_tokens[i] .. cu_tokens[i + 1] - 1 of key / value fp16 [T, HK, D]
+    (int32 [S + 1]; None: one token per sequence) and take its positions context_lens[i] - n ..
+    context_lens[i] - 1: context_lens [S] already counts them, as the attention call that follows reads it.
+    k_scale_per_block / v_scale_per_block (float32 [num_blocks, HK]) are read and written: a block's scale
+    grows to max|row| / q of its new rows where that is more (q = 127, 448 or 57344 for int8, e4m3, e5m2), the
+    rows held before are then stored again under the new scale, and a block whose first row is new starts
+    afresh.  A block of zeros has scale 0.  Infinities count as the largest fp16 value, NaNs do not count.
+
+    With `cos_sin` (see `rope_and_cache`) K is rotated by its position on the way, and query -> query_out too
+    if given.  The blocks a call writes must belong to one sequence each (full blocks may be shared).  Rows
+    behind the last sequence, and tokens whose position lies outside the table row or the rotation table, are
+    skipped.  Asynchronous on torch's current stream.
+    """
+    _check_caches(key, value, key_cache, value_cache)
+    device = key_cache.device
+    p = _cabi.PaBlockScaledParams()
+    p.key_token_stride = _token_rows(key, "key", device)
+    p.value_token_stride = _token_rows(value, "value", device)
+    nb, bs, hk, d = key_cache.shape
+    for name, t in (("k_scale_per_block", k_scale_per_block), ("v_scale_per_block", v_scale_per_block)):
+        _require(t.dtype == torch.float32 and tuple(t.shape) == (nb, hk) and t.is_contiguous() and t.device == device,
+                 f"{name} must be a contiguous float32 tensor [num_blocks, num_kv_heads] on the cache's device")
+    _require(block_tables.dim() == 2 and block_tables.size(0) == context_lens.numel(),
+             "block_tables must be [num_seqs, max_blocks_per_seq] with one context length per row")
+    for name, t in (("block_tables", block_tables), ("context_lens", context_lens), ("cu_tokens", cu_tokens)):
+        _require(t is None or (t.dtype == torch.int32 and t.is_contiguous() and t.device == device),
+                 f"{name} must be contiguous int32 on the cache's device")
+    seqs = context_lens.numel()
+    _require(cu_tokens is None or cu_tokens.numel() == seqs + 1, "cu_tokens must have num_seqs + 1 entries")
+    _require(query is None or cos_sin is not None, "queries are only taken to be rotated: cos_sin is missing")
+    if cos_sin is not None:
+        _check_rotation(cos_sin, device)
+        p.cos_sin, p.max_position, p.rotary_dim = cos_sin.data_ptr(), cos_sin.size(0), cos_sin.size(1)
+    _check_queries(p, query, query_out, key)
+    p.key, p.value = key.data_ptr(), value.data_ptr()
+    p.key_cache, p.value_cache = key_cache.data_ptr(), value_cache.data_ptr()
+    p.k_scale_per_block, p.v_scale_per_block = k_scale_per_block.data_ptr(), v_scale_per_block.data_ptr()
+    p.block_tables, p.context_lens = block_tables.data_ptr(), context_lens.data_ptr()
+    p.cu_tokens = cu_tokens.data_ptr() if cu_tokens is not None else None
+    p.num_seqs, p.num_tokens, p.num_kv_heads, p.head_size = seqs, key.size(0), hk, d
+    p.block_size, p.max_blocks_per_seq, p.num_blocks = bs, block_tables.size(1), nb
+    p.kv_dtype, p.interleaved = _kv_dtype(key_cache), int(interleaved)
+    _call(_cabi.load_library().pa_append_block_scaled, p, device)

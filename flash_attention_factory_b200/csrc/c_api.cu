@@ -10,6 +10,9 @@ int read_status_fp8_loop(int *v);
 int read_status_fp8_reduce(int *v);
 int read_status_int8_loop(int *v);
 int read_status_int8_reduce(int *v);
+int read_status_diff(int *v);
+int read_status_diff_fp8(int *v);
+int read_status_diff_int8(int *v);
 
 } // namespace pa
 
@@ -56,7 +59,8 @@ PA_API int pa_device_status(void) {
   cudaError_t err = cudaDeviceSynchronize();
   if (err != cudaSuccess) return pa::fail(PA_ERR_CUDA, "cudaDeviceSynchronize failed: %s", cudaGetErrorString(err));
   int (*readers[])(int *) = {pa::read_status_loop,       pa::read_status_reduce,    pa::read_status_fp8_loop,
-                             pa::read_status_fp8_reduce, pa::read_status_int8_loop, pa::read_status_int8_reduce};
+                             pa::read_status_fp8_reduce, pa::read_status_int8_loop, pa::read_status_int8_reduce,
+                             pa::read_status_diff,       pa::read_status_diff_fp8,  pa::read_status_diff_int8};
   int worst = 0;
   for (auto reader : readers) {
     int v = 0;

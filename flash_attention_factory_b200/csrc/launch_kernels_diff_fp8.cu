@@ -1,0 +1,11 @@
+// Attention kernel of launch_kernels_diff for FP8 caches (see launch_kernels_diff.cu).
+#include "differential_attention.cuh"
+
+namespace pa {
+int read_status_diff_fp8(int *v) { return read_and_clear_device_status(v); }
+int enqueue_diff_e5m2(const pa_params *p, cudaStream_t stream) { return dispatch_diff<KV_E5M2>(p, stream); }
+int enqueue_diff_e4m3(const pa_params *p, cudaStream_t stream) { return dispatch_diff<KV_E4M3>(p, stream); }
+} // namespace pa
+
+PA_TIMELINE_ACCESSOR(pa_debug_timeline_diff_fp8)
+PA_BOUNDS_ACCESSOR(pa_debug_bounds_diff_fp8)

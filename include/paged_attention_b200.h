@@ -186,6 +186,42 @@ PA_API int launch_kernels_fp8_reduce(const pa_params *p, void *stream, float *us
 PA_API int launch_kernels_int8_loop(const pa_params *p, void *stream, float *us_out);
 PA_API int launch_kernels_int8_reduce(const pa_params *p, void *stream, float *us_out);
 
+/* Arguments of launch_kernels_diff.  `attn` is the ordinary argument block with these meanings:
+ *   num_heads      2 H: head h of the result has its two query maps at rows 2 h and 2 h + 1
+ *   num_kv_heads   2 HK: KV pair k holds its two K heads at 2 k and 2 k + 1 and its value vector
+ *                  of 2 * head_size elements as V heads 2 k and 2 k + 1 side by side, so both
+ *                  caches keep the layout [num_blocks, block_size, 2 HK, head_size] and every
+ *                  cache writer of this library fills them
+ *   num_queries_per_tokens  H / HK, 1..8
+ *   out            fp16 [num_seqs, H, 2 * head_size]
+ *   max_logits, exp_sums    fp32 [num_seqs, 2 H, max_num_partitions]
+ *   tmp_out        fp32 [num_seqs, 2 H, max_num_partitions, 2 * head_size]
+ *   kv_dtype       any pa_kv_dtype; scales as in the FP8 and int8 entry points, per cache head
+ *   sinks, alibi_slopes, softcap  must be off
+ * A context is cut into at most max_num_partitions partitions of P tokens, P the smallest power of two
+ * from 64 on with P * max_num_partitions >= max_context_len; the last one is open-ended, so the result
+ * never depends on max_context_len. */
+typedef struct pa_diff_params {
+  pa_params attn;
+  const float *lambdas;     /* fp32 [H]: the learned weight of the second map */
+  const float *norm_weight; /* fp32 [2 * head_size], or NULL: no norm */
+  float norm_eps;           /* > 0 where norm_weight is set */
+  float norm_scale;         /* constant factor of the normed row (1 - lambda_init) */
+} pa_diff_params;
+
+/* Differential attention of one decode token per sequence (no reference counterpart):
+ *   o[h] = (softmax(s q[2h] . K[2k]) - lambdas[h] * softmax(s q[2h+1] . K[2k+1])) . [V[2k] V[2k+1]],
+ * k = h / (H / HK), s = sm_scale, then, with norm_weight w,
+ *   o[h] <- o[h] / sqrt(mean(o[h]^2) + norm_eps) * w * norm_scale.
+ * An empty context gives zeros.  us_out[0] = attention kernel, us_out[1] = merge kernel. */
+PA_API int launch_kernels_diff(const pa_diff_params *p, void *stream, float *us_out);
+
+/* Partitions that launch_kernels_diff is fastest with (the max_num_partitions to size its scratch
+ * for): 512-token partitions, shorter ones while the batch does not fill the GPU.  num_kv_heads is
+ * that of the cache (2 HK); 0 if the head size or an odd number of KV heads is not supported. */
+PA_API uint32_t pa_diff_num_partitions(uint32_t num_seqs, uint32_t num_kv_heads, uint32_t head_size,
+                                       uint32_t max_context_len);
+
 /* Size in bytes of the scratch array built into the library for
  * launch_kernels_reduce_static_scratch (32 MiB, held by every GPU that loads the library). */
 #define PA_STATIC_SCRATCH_BYTES (32u * 1024u * 1024u)
@@ -420,6 +456,53 @@ typedef struct pa_rope_cache_params {
  * outside the cache, or whose position is outside the table, is skipped altogether: its cache and
  * query_out rows stay as they were.  Slots of one call have to differ.  head_size: a multiple of 16. */
 PA_API int pa_rope_and_cache(const pa_rope_cache_params *p, void *stream);
+
+/* Arguments of pa_append_block_scaled. */
+typedef struct pa_block_scaled_params {
+  const void *key;              /* fp16 rows of [num_kv_heads, head_size], key_token_stride apart */
+  const void *value;
+  void *key_cache;              /* [num_blocks, block_size, num_kv_heads, head_size], int8 or FP8 */
+  void *value_cache;
+  float *k_scale_per_block;     /* fp32 [num_blocks, num_kv_heads], read and written */
+  float *v_scale_per_block;
+  const uint32_t *block_tables; /* [num_seqs, max_blocks_per_seq] */
+  const uint32_t *context_lens; /* [num_seqs], the new tokens included */
+  const uint32_t *cu_tokens;    /* [num_seqs + 1]: sequence i's new tokens are rows cu_tokens[i] ..
+                                   cu_tokens[i + 1] - 1; NULL: one token per sequence */
+  uint32_t num_seqs;
+  uint32_t num_tokens;          /* rows of key and value */
+  uint32_t num_kv_heads;
+  uint32_t head_size;           /* a multiple of 16, at most 512 */
+  uint32_t block_size;
+  uint32_t max_blocks_per_seq;
+  uint64_t num_blocks;
+  int32_t kv_dtype;             /* PA_KV_INT8, PA_KV_FP8_E4M3 or PA_KV_FP8_E5M2 */
+  uint32_t interleaved;
+  /* optional rotation of K (and of the queries), as in pa_rope_and_cache; the position of a token is
+   * its place in its sequence */
+  const float *cos_sin;         /* fp32 [max_position, rotary_dim], or NULL: no rotation */
+  uint64_t max_position;
+  uint32_t rotary_dim;
+  uint32_t num_heads;
+  const void *query;
+  void *query_out;
+  uint64_t query_token_stride;
+  uint64_t key_token_stride;
+  uint64_t value_token_stride;
+} pa_block_scaled_params;
+
+/* Appends new K/V tokens to an 8-bit cache that keeps one scale for each block of tokens and KV head,
+ * and keeps those scales (no reference counterpart; the arrays are the ones the attention entry points
+ * read as k_scale_per_block / v_scale_per_block).  The n new tokens of a sequence take its positions
+ * context_len - n .. context_len - 1.  For every block and head they reach, K and V each:
+ *   s' = max(s, max|new rows| / q), s = 0 if the block's first row is among the new ones,
+ *   q = 127 (int8), 448 (e4m3), 57344 (e5m2);
+ * where s' > s the rows held before are stored again as code' = round(code * s / s'), and the new rows
+ * are stored as round(x / s'), x the (rotated) fp32 value.  Rows behind the context stay as they were.
+ * A block of zeros has scale 0.  Infinite inputs count as the largest fp16 value, NaNs do not count.
+ * The blocks that a call writes must belong to one sequence each.  A token outside its table row, a block
+ * id >= num_blocks, or a position outside the rotation table: the token is skipped. */
+PA_API int pa_append_block_scaled(const pa_block_scaled_params *p, void *stream);
 
 /* Compile-time policy of include/paged_attention_policy_v2.hpp as data
  * (reference include/paged_attention_policy_v2.hpp:5-100).  Returns

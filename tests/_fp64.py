@@ -26,14 +26,17 @@ def sequence(values, table_row, n):
     return values[ids].flatten(0, 1)[:n]
 
 
-def attention64(case, k_scale=None, v_scale=None, sinks=None, softcap=0.0, alibi=None):
+def attention64(case, k_scale=None, v_scale=None, sinks=None, softcap=0.0, alibi=None, weighted_code=0.0):
     """(result, allowed error) [S, H, D] of decode attention in fp64.
 
     Allowed error, |v| weighted by the softmax being a = sum_t p_t |v_t|: the weights are rounded
     to fp16 before the value product (HALF a), the split variant stores partial rows in fp16 (HALF a),
     the result is fp16 (HALF a at most), and the fp32 chains (dot products of at most 128 terms,
     exponentials, sums) stay below another HALF a; a weight under 2^-14 of the reference is
-    subnormal and off by up to 2^-25 absolute, of a reference of at least 1: n 2^-25 max|v|."""
+    subnormal and off by up to 2^-25 absolute, of a reference of at least 1: n 2^-25 max|v|.
+    `weighted_code`: the largest code where a block's V scale is multiplied into the weights as it is
+    (the FP8 operators): the product p scale is then what is rounded, off by up to 2^-25 absolute where
+    it is subnormal, and meets a code c instead of a value: n 2^-25 max|c|, 448 for e4m3."""
     q, bt, lens = case["query"].double(), case["block_tables"], [int(c) for c in case["context_lens"]]
     kv, vv = cache_values(case["key_cache"], k_scale), cache_values(case["value_cache"], v_scale)
     s, h, d = q.shape
@@ -53,7 +56,7 @@ def attention64(case, k_scale=None, v_scale=None, sinks=None, softcap=0.0, alibi
         p = torch.softmax(sc, dim=-1)[..., :n]
         out[i] = torch.einsum("kgt,tkd->kgd", p, v).reshape(h, d)
         a = torch.einsum("kgt,tkd->kgd", p, v.abs()).reshape(h, d)
-        tol[i] += 4 * HALF * a + n * 2.0 ** -25 * v.abs().max()
+        tol[i] += 4 * HALF * a + n * 2.0 ** -25 * max(float(v.abs().max()), weighted_code)
     return out, tol
 
 

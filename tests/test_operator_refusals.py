@@ -122,3 +122,68 @@ def test_cache_ops_refuse_cpu_tensors_and_odd_layouts():
     i = torch.zeros(2, dtype=torch.int64)
     with pytest.raises(RuntimeError, match="CUDA"):
         cache_ops.rope_and_cache(None, k, k, i, torch.zeros(4, 64), None, kc, kc, i)
+
+
+def test_append_block_scaled(lib):
+    def call(**kw):
+        p = _cabi.PaBlockScaledParams()
+        base = dict(key=0x1000, value=0x2000, key_cache=0x3000, value_cache=0x4000, k_scale_per_block=0x5000,
+                    v_scale_per_block=0x6000, block_tables=0x7000, context_lens=0x8000, num_seqs=3, num_tokens=3,
+                    num_kv_heads=2, head_size=128, block_size=16, max_blocks_per_seq=4, num_blocks=8, kv_dtype=_cabi.KV_INT8,
+                    key_token_stride=256, value_token_stride=256)
+        base.update(kw)
+        for k, v in base.items():
+            setattr(p, k, v)
+        return lib.pa_append_block_scaled(ctypes.byref(p), None), lib.pa_last_error().decode()
+
+    bad, unsupported = _cabi.PA_ERR_BAD_ARG, _cabi.PA_ERR_UNSUPPORTED
+    assert lib.pa_append_block_scaled(None, None) == bad
+    assert call(num_tokens=0)[0] == _cabi.PA_OK and call(num_seqs=0)[0] == _cabi.PA_OK
+    assert call(kv_dtype=_cabi.KV_F16)[0] == bad and call(kv_dtype=7)[0] == bad
+    assert call(head_size=72)[0] == unsupported
+    assert call(block_size=24)[0] == unsupported and call(block_size=2048)[0] == unsupported
+    assert call(num_kv_heads=0)[0] == bad
+    for name in ("key", "value", "key_cache", "value_cache", "k_scale_per_block", "v_scale_per_block", "block_tables", "context_lens"):
+        rc, msg = call(**{name: 0})
+        assert rc == bad and "null" in msg, name
+    assert "num_tokens must equal" in call(num_tokens=4)[1]
+    assert call(key=0x1008)[0] == bad
+    assert call(num_blocks=0)[0] == bad
+    assert call(cos_sin=0x9000, max_position=8, rotary_dim=40)[0] == unsupported
+    assert "together" in call(query=0xa000)[1]
+
+
+def test_differential_attention(lib):
+    def call(lambdas=0x1000, norm_weight=0, norm_eps=1e-5, **kw):
+        p = _cabi.PaDiffParams()
+        src = _attn(**{"kv_dtype": _cabi.KV_F16, **kw})
+        ctypes.memmove(ctypes.byref(p.attn), ctypes.byref(src), ctypes.sizeof(src))
+        p.lambdas, p.norm_weight, p.norm_eps, p.norm_scale = lambdas, norm_weight, norm_eps, 1.0
+        return lib.launch_kernels_diff(ctypes.byref(p), None, None), lib.pa_last_error().decode()
+
+    bad, unsupported = _cabi.PA_ERR_BAD_ARG, _cabi.PA_ERR_UNSUPPORTED
+    assert lib.launch_kernels_diff(None, None, None) == bad
+    assert call(num_seqs=0)[0] == _cabi.PA_OK
+    assert call(kv_dtype=8)[0] == bad
+    assert call(head_size=96)[0] == unsupported
+    assert call(num_queries_per_tokens=9, num_heads=18)[0] == unsupported
+    rc, msg = call(num_heads=12, num_kv_heads=3)
+    assert rc == bad and "pairs" in msg
+    assert call(lambdas=0)[0] == bad
+    assert call(norm_weight=0x1000, norm_eps=0.0)[0] == bad
+    assert call(norm_weight=0x1004)[0] == bad
+    for extra in (dict(sinks=0x1000), dict(alibi_slopes=0x1000), dict(softcap=3.0)):
+        assert call(**extra)[0] == unsupported
+    assert call(max_logits=0)[0] == bad and call(max_num_partitions=0)[0] == bad
+    assert call(k_scale_per_head=0x1000, v_scale_per_head=0x1000)[0] == bad  # an fp16 cache has no scales
+
+
+def test_diff_partition_counts(lib):
+    n = lib.pa_diff_num_partitions
+    assert n(1, 3, 128, 1000) == 0 and n(1, 2, 96, 1000) == 0 and n(1, 0, 128, 1000) == 0
+    assert n(4, 8, 128, 0) == 1 and n(4, 8, 128, 1) == 1
+    assert n(1000, 8, 128, 1024) == 2       # a batch that fills the GPU: 512-token partitions
+    assert n(1, 2, 64, 1000) == 16          # a lone short sequence: the shortest ones
+    assert n(1, 8, 128, 2 ** 31) == 65535
+    sizes = [n(2, 8, 128, c) for c in range(1, 5000, 97)]
+    assert all(64 * s >= c for s, c in zip(sizes, range(1, 5000, 97)) if s < 65535)
