@@ -293,7 +293,7 @@ def load_library() -> ctypes.CDLL:
         fn.restype = ctypes.c_int
     lib.launch_kernels_diff.argtypes = [ctypes.POINTER(PaDiffParams), ctypes.c_void_p, ctypes.POINTER(ctypes.c_float)]
     lib.launch_kernels_diff.restype = ctypes.c_int
-    lib.pa_diff_num_partitions.argtypes = [ctypes.c_uint32] * 4
+    lib.pa_diff_num_partitions.argtypes = [ctypes.c_uint32] * 4 + [ctypes.c_int32]
     lib.pa_diff_num_partitions.restype = ctypes.c_uint32
     lib.launch_kernels_reduce_static_scratch.argtypes = [ctypes.POINTER(PaParams), ctypes.c_void_p]
     lib.launch_kernels_reduce_static_scratch.restype = ctypes.c_int

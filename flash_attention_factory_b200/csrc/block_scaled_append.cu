@@ -28,6 +28,8 @@ struct AppendArgs {
   uint32_t num_seqs, num_tokens, num_heads, num_kv_heads, head_size, block_shift, block_size, max_blocks_per_seq;
   uint32_t rotary_dim;
   uint32_t tokens_per_cta; // 1..32
+  uint32_t warps_per_job;  // 1, 2, 4 or 8
+  uint32_t append_ctas;    // CTAs of a column that append; the others rotate queries
 };
 
 template <int KV>
@@ -44,22 +46,37 @@ struct TokenPlace {
   bool leads;         // first new token of its block
 };
 
-// Sequence of a token by bisection of the row offsets, then its position, block and neighbours.
-__device__ __forceinline__ TokenPlace place_token(const AppendArgs &a, uint32_t token) {
+// Sequence of this lane's token: the last entry of the row offsets that is not beyond it.  The warp holds every
+// step-th offset in registers and bisects those with shuffles; what is left of the search (nothing up to
+// 31 sequences) goes to memory.  Returns num_seqs for a token of no sequence.  Called by all lanes.
+__device__ __forceinline__ uint32_t find_sequence(const AppendArgs &a, uint32_t token, uint32_t lane) {
+  const uint32_t n = a.num_seqs + 1u;
+  const uint32_t step = (n + 31u) / 32u;
+  const uint32_t sample = (lane * step < n) ? __ldg(a.cu_tokens + lane * step) : 0xffffffffu;
+  uint32_t k = 0; // samples that are not beyond the token, at most 31
+#pragma unroll
+  for (uint32_t b = 16; b > 0; b >>= 1)
+    if (__shfl_sync(0xffffffffu, sample, k + b - 1u) <= token) k += b;
+  if (__shfl_sync(0xffffffffu, sample, 31) <= token) k = 32;
+  if (k == 0) return a.num_seqs;
+  uint32_t lo = (k - 1u) * step, hi = min(lo + step, n); // the entry lies in [lo, hi)
+  while (hi - lo > 1u) {
+    const uint32_t mid = (lo + hi) >> 1;
+    if (__ldg(a.cu_tokens + mid) <= token) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// Place of this lane's token: sequence, position, block and the tokens that follow it there.  Called by all lanes.
+__device__ __forceinline__ TokenPlace place_token(const AppendArgs &a, uint32_t token, bool mine, uint32_t lane) {
   TokenPlace t{};
-  if (token >= a.num_tokens) return t;
   uint32_t seq = token, begin = token, end = token + 1;
+  if (a.cu_tokens != nullptr) seq = find_sequence(a, token, lane);
+  if (!mine || token >= a.num_tokens || seq >= a.num_seqs) return t;
   if (a.cu_tokens != nullptr) {
-    uint32_t lo = 0, hi = a.num_seqs + 1; // first offset beyond the token
-    while (lo < hi) {
-      const uint32_t mid = (lo + hi) >> 1;
-      if (__ldg(a.cu_tokens + mid) <= token) lo = mid + 1;
-      else hi = mid;
-    }
-    if (lo == 0 || lo > a.num_seqs) return t; // before the first or behind the last sequence
-    seq = lo - 1;
     begin = __ldg(a.cu_tokens + seq);
-    end = min(__ldg(a.cu_tokens + lo), a.num_tokens);
+    end = min(__ldg(a.cu_tokens + seq + 1), a.num_tokens);
   }
   const int64_t position = static_cast<int64_t>(__ldg(a.context_lens + seq)) - (end - token);
   if (position < 0 || static_cast<uint64_t>(position) >= a.position_limit) return t;
@@ -67,106 +84,263 @@ __device__ __forceinline__ TokenPlace place_token(const AppendArgs &a, uint32_t 
   t.block = __ldg(a.block_tables + static_cast<size_t>(seq) * a.max_blocks_per_seq + (t.position >> a.block_shift));
   if (t.block >= a.num_blocks) return t;
   const uint32_t row = t.position & (a.block_size - 1u);
-  t.leads = row == 0 || token == begin || t.position == 0;
+  t.leads = row == 0 || token == begin;
   const uint64_t room = min(static_cast<uint64_t>(a.block_size - row), a.position_limit - t.position);
   t.rows_here = static_cast<uint32_t>(min(room, static_cast<uint64_t>(end - token)));
   t.valid = true;
   return t;
 }
 
-// One warp: K or V rows [0, rows) of one (block, head), rows laid over the lanes in items of 16 elements.
-template <int KV, bool INTERLEAVED>
-__device__ void append_rows(const AppendArgs &a, const __half *src, uint64_t stride, bool rotate, uint32_t position,
-                            uint8_t *block_rows, float *scale_at, uint32_t first_row, uint32_t rows, uint32_t lane) {
-  const uint32_t D = a.head_size;
-  const uint32_t lanes_per_row = D / 16u;
-  const uint32_t rows_per_pass = 32u / lanes_per_row;
-  const uint32_t item = lane % lanes_per_row, lane_row = lane / lanes_per_row;
-  const bool active = lane_row < rows_per_pass;
-  const RotaryItem rot = rotate ? rotary_item(item, a.rotary_dim, INTERLEAVED) : rotary_item(item, 0u, false);
-  const size_t pitch = static_cast<size_t>(a.num_kv_heads) * D; // bytes between two rows of the block
+constexpr uint32_t kAppendThreads = 256;
+constexpr uint32_t kAppendWarps = kAppendThreads / 32;
 
-  auto load_row = [&](uint32_t r, float (&x)[8], float (&y)[8]) {
-    const __half *row = src + static_cast<size_t>(r) * stride;
-    unpack_half8(__ldg(reinterpret_cast<const uint4 *>(row + rot.first)), x);
-    unpack_half8(__ldg(reinterpret_cast<const uint4 *>(row + rot.second)), y);
-    // infinities count as the largest fp16 value, so that one of them does not take the block's scale
+// What a lane does of every row group: the lanes of a warp hold rows_per_pass rows side by side, 16 elements
+// each (see rotary_item).
+struct LaneShare {
+  uint32_t item, row, rows_per_pass;
+  bool active;
+  __device__ __forceinline__ LaneShare(uint32_t head_size, uint32_t lane) {
+    const uint32_t lanes_per_row = head_size / 16u;
+    rows_per_pass = 32u / lanes_per_row;
+    item = lane % lanes_per_row;
+    row = lane / lanes_per_row;
+    active = row < rows_per_pass;
+  }
+};
+
+// What one warp does for K or V of one (block, head): some of its new rows.
+struct RowJob {
+  const __half *src;   // the warp's first row
+  uint64_t stride;     // elements between two rows
+  const float *angles; // rotation table row of that row; null: not rotated
+  uint8_t *dst;        // where that row goes
+  size_t pitch;        // bytes between two rows of the block
+  uint32_t rows;
+  uint32_t rotary_dim;
+};
+
+// The general way, row by row from memory: rows with infinities or NaNs (an infinity counts as the largest fp16
+// value, so that it does not take the block's scale; NaNs drop out of fmaxf), and more rows than a warp keeps
+// in registers.
+template <bool INTERLEAVED>
+__device__ __forceinline__ void load_row_with_care(const RowJob &job, const LaneShare &l, const RotaryItem &rot, uint32_t r,
+                                                   float (&x)[8], float (&y)[8]) {
+  const __half *row = job.src + static_cast<size_t>(r) * job.stride;
+  unpack_half8(__ldg(reinterpret_cast<const uint4 *>(row + rot.first)), x);
+  unpack_half8(__ldg(reinterpret_cast<const uint4 *>(row + rot.second)), y);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (isinf(x[j])) x[j] = copysignf(65504.f, x[j]);
-      if (isinf(y[j])) y[j] = copysignf(65504.f, y[j]);
-    }
-    if (rot.rotated) {
-      float c[8], s[8];
-      load_cos_sin(a.cos_sin + static_cast<size_t>(position + r) * a.rotary_dim, item, a.rotary_dim, c, s);
-      rotate_item(x, y, c, s, INTERLEAVED);
-    }
-  };
+  for (int j = 0; j < 8; ++j) {
+    if (isinf(x[j])) x[j] = copysignf(65504.f, x[j]);
+    if (isinf(y[j])) y[j] = copysignf(65504.f, y[j]);
+  }
+  if (rot.rotated) {
+    float c[8], s[8];
+    load_cos_sin(job.angles + static_cast<size_t>(r) * job.rotary_dim, l.item, job.rotary_dim, c, s);
+    rotate_item(x, y, c, s, INTERLEAVED);
+  }
+}
 
-  const float held = (first_row == 0u) ? 0.f : *scale_at;
-  float top = 0.f; // NaNs drop out of fmaxf
-  for (uint32_t r = lane_row; active && r < rows; r += rows_per_pass) {
+template <bool INTERLEAVED>
+__device__ __forceinline__ float largest_with_care(const RowJob &job, const LaneShare &l) {
+  const RotaryItem rot = rotary_item(l.item, job.angles != nullptr ? job.rotary_dim : 0u, INTERLEAVED);
+  float top = 0.f;
+#pragma unroll 1
+  for (uint32_t r = l.row; l.active && r < job.rows; r += l.rows_per_pass) {
     float x[8], y[8];
-    load_row(r, x, y);
+    load_row_with_care<INTERLEAVED>(job, l, rot, r, x, y);
 #pragma unroll
     for (int j = 0; j < 8; ++j) top = fmaxf(top, fmaxf(fabsf(x[j]), fabsf(y[j])));
   }
-#pragma unroll
-  for (uint32_t o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float scale = fmaxf(held, __fdiv_rn(top, largest_code<KV>()));
-  const float by = (scale > 0.f) ? scale : 1.f; // a block of zeros keeps scale 0 and codes 0
+  return top;
+}
 
-  if (scale > held && active) {
-    // the rows held before, under the new scale
-    for (uint32_t r = lane_row; r < first_row; r += rows_per_pass) {
-      uint4 *at = reinterpret_cast<uint4 *>(block_rows + r * pitch + item * 16u);
-      uint4 v = *at;
-      uint32_t *w = reinterpret_cast<uint32_t *>(&v);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float x[4];
-        unpack_codes<KV>(w[i], x);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = __fdiv_rn(__fmul_rn(x[j], held), by);
-        w[i] = pack_codes<KV>(x[0], x[1], x[2], x[3]);
-      }
-      *at = v;
-    }
-  }
-  for (uint32_t r = lane_row; active && r < rows; r += rows_per_pass) {
+template <int KV, bool INTERLEAVED>
+__device__ __forceinline__ void store_with_care(const RowJob &job, const LaneShare &l, float scale) {
+  const RotaryItem rot = rotary_item(l.item, job.angles != nullptr ? job.rotary_dim : 0u, INTERLEAVED);
+  const Divider by(scale);
+#pragma unroll 1
+  for (uint32_t r = l.row; l.active && r < job.rows; r += l.rows_per_pass) {
     float x[8], y[8];
-    load_row(r, x, y);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      x[j] = __fdiv_rn(x[j], by);
-      y[j] = __fdiv_rn(y[j], by);
-    }
-    uint8_t *row = block_rows + (first_row + r) * pitch;
+    load_row_with_care<INTERLEAVED>(job, l, rot, r, x, y);
+    divide8(x, by);
+    divide8(y, by);
+    uint8_t *row = job.dst + r * job.pitch;
     *reinterpret_cast<uint2 *>(row + rot.first) =
         make_uint2(pack_codes<KV>(x[0], x[1], x[2], x[3]), pack_codes<KV>(x[4], x[5], x[6], x[7]));
     *reinterpret_cast<uint2 *>(row + rot.second) =
         make_uint2(pack_codes<KV>(y[0], y[1], y[2], y[3]), pack_codes<KV>(y[4], y[5], y[6], y[7]));
   }
-  __syncwarp(); // every lane has read the old scale
-  if (lane == 0) *scale_at = scale;
 }
 
-// A CTA owns tokens_per_cta consecutive new tokens: it appends the blocks whose first new token is among
-// them (a block belongs to exactly one CTA whatever its later tokens) and rotates the tokens' queries.
-// Every warp works out the places of the tokens for itself, a token per lane, and takes every n-th
-// (head, K or V) of a block.
-template <int KV, bool INTERLEAVED>
-__global__ void __launch_bounds__(512) append_block_scaled_kernel(const AppendArgs a) {
+// Rows that a block held before, under its new scale; 16 codes of every row for this lane.
+template <int KV>
+__device__ __forceinline__ void requantise_rows(uint8_t *at, size_t step, uint32_t rows, float held, float scale) {
+#pragma unroll 1
+  for (uint32_t r = 0; r < rows; ++r, at += step) {
+    uint4 v = *reinterpret_cast<uint4 *>(at);
+    uint32_t *w = reinterpret_cast<uint32_t *>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float c[4];
+      unpack_codes<KV>(w[i], c);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) c[j] = __fdiv_rn(__fmul_rn(c[j], held), scale);
+      w[i] = pack_codes<KV>(c[0], c[1], c[2], c[3]);
+    }
+    *reinterpret_cast<uint4 *>(at) = v;
+  }
+}
+
+// The usual way: up to PASSES row groups of the warp live in registers as they came (fp16), read once, and are written
+// from there when the scale is known.  K is rotated twice, once for the maximum and once for the codes: keeping
+// the rotated rows as fp32 would take twice the registers, which spilled.  The maximum of V is taken two fp16
+// values at a time.  The maxima propagate NaNs, so an infinity or a NaN among the inputs shows in the result.
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+template <int PASSES, bool ROTATE, bool INTERLEAVED>
+struct HeldRows {
+  uint4 raw[PASSES][2];
+
+  // the fp32 values of one row group, K rotated
+  __device__ __forceinline__ void values(int i, const RowJob &job, const LaneShare &l, const RotaryItem &rot, int valid,
+                                         float (&x)[8], float (&y)[8]) const {
+    unpack_half8(raw[i][0], x);
+    unpack_half8(raw[i][1], y);
+    if constexpr (ROTATE) {
+      if (rot.rotated && i < valid) {
+        float c[8], s[8];
+        load_cos_sin(job.angles + static_cast<size_t>(l.row + i * l.rows_per_pass) * job.rotary_dim, l.item, job.rotary_dim, c, s);
+        rotate_item(x, y, c, s, INTERLEAVED);
+      }
+    }
+  }
+
+  // reads the rows; returns their largest magnitude
+  __device__ __forceinline__ float load(const RowJob &job, const LaneShare &l, const RotaryItem &rot, int valid) {
+    const __half *at = job.src + static_cast<size_t>(l.row) * job.stride;
+    const size_t step = l.rows_per_pass * job.stride;
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      raw[i][0] = raw[i][1] = make_uint4(0u, 0u, 0u, 0u); // rows past the end as zeros
+      if (i < valid) {
+        raw[i][0] = __ldg(reinterpret_cast<const uint4 *>(at + i * step + rot.first));
+        raw[i][1] = __ldg(reinterpret_cast<const uint4 *>(at + i * step + rot.second));
+      }
+    }
+    if constexpr (ROTATE) {
+      float top = 0.f;
+#pragma unroll
+      for (int i = 0; i < PASSES; ++i) {
+        float x[8], y[8];
+        values(i, job, l, rot, valid, x, y);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = max_or_nan(top, max_or_nan(fabsf(x[j]), fabsf(y[j])));
+      }
+      return top;
+    } else {
+      __half2 top = __half2half2(__ushort_as_half(0));
+#pragma unroll
+      for (int i = 0; i < PASSES; ++i) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const __half2 *h = reinterpret_cast<const __half2 *>(&raw[i][k]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) top = __hmax2_nan(top, __habs2(h[j]));
+        }
+      }
+      const float2 t = __half22float2(top);
+      return max_or_nan(t.x, t.y);
+    }
+  }
+
+  template <int KV>
+  __device__ __forceinline__ void store(const RowJob &job, const LaneShare &l, const RotaryItem &rot, int valid, float scale) const {
+    const Divider by(scale); // the caller has made sure of its range
+    uint8_t *at = job.dst + l.row * job.pitch;
+    const size_t step = l.rows_per_pass * job.pitch;
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      float x[8], y[8];
+      values(i, job, l, rot, valid, x, y);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        x[j] = by(x[j]);
+        y[j] = by(y[j]);
+      }
+      if (i < valid) {
+        *reinterpret_cast<uint2 *>(at + i * step + rot.first) =
+            make_uint2(pack_small_codes<KV>(x[0], x[1], x[2], x[3]), pack_small_codes<KV>(x[4], x[5], x[6], x[7]));
+        *reinterpret_cast<uint2 *>(at + i * step + rot.second) =
+            make_uint2(pack_small_codes<KV>(y[0], y[1], y[2], y[3]), pack_small_codes<KV>(y[4], y[5], y[6], y[7]));
+      }
+    }
+  }
+};
+
+// K (ROTATE) or V rows of one (block, head) by `parts` warps, of which this is number `part`.
+template <int KV, bool INTERLEAVED, int PASSES, bool ROTATE>
+__device__ __forceinline__ void append_rows(const RowJob &job, const LaneShare &l, bool live, uint32_t part, uint32_t parts,
+                                            uint32_t first_row, uint8_t *block_rows, float *scale_at, float *tops,
+                                            uint32_t lane, uint32_t warp) {
+  const RotaryItem rot = rotary_item(l.item, ROTATE ? job.rotary_dim : 0u, INTERLEAVED);
+  const bool in_registers = job.rows <= PASSES * l.rows_per_pass;
+  int valid = 0; // row groups that hold a row for this lane
+  if (l.active && live && l.row < job.rows) valid = static_cast<int>((job.rows - l.row + l.rows_per_pass - 1u) / l.rows_per_pass);
+  const float held = (live && first_row != 0u) ? *scale_at : 0.f;
+  HeldRows<PASSES, ROTATE, INTERLEAVED> kept;
+  bool careful = true;
+  float top = 0.f;
+  if (in_registers) {
+    top = kept.load(job, l, rot, valid);
+    careful = __any_sync(0xffffffffu, !(top <= 1e30f)) != 0;
+  }
+  if (careful && live) top = largest_with_care<INTERLEAVED>(job, l);
+  top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))); // magnitudes order like their bits
+  if (parts > 1u) { // the largest value of the job's warps
+    if (lane == 0) tops[warp] = top;
+    __syncthreads();
+    for (uint32_t k = 0; k < parts; ++k) top = fmaxf(top, tops[warp - part + k]);
+  }
+  if (!live) return;
+  const float grown = fmaxf(held, __fdiv_rn(top, largest_code<KV>()));
+  const float scale = (grown > 0.f) ? grown : 1.f; // a block of zeros keeps scale 0 and codes 0
+  if (!careful && !Divider(scale).plain) kept.template store<KV>(job, l, rot, valid, scale);
+  else store_with_care<KV, INTERLEAVED>(job, l, scale);
+  if (grown > held && l.active) {
+    const uint32_t r = part * l.rows_per_pass + l.row, step = parts * l.rows_per_pass;
+    if (r < first_row)
+      requantise_rows<KV>(block_rows + r * job.pitch + l.item * 16u, step * job.pitch, divide_round_up(first_row - r, step), held,
+                          scale);
+  }
+  __syncwarp(); // every lane has read the old scale; the job's other warps read it before the barrier above
+  if (lane == 0 && part == 0u) *scale_at = grown;
+}
+
+// A column of CTAs (blockIdx.x) owns tokens_per_cta consecutive new tokens: it appends the blocks whose first new
+// token is among them (a block belongs to exactly one column whatever its later tokens) and rotates the tokens'
+// queries.  The jobs of a block (K and V of each head) go round the warps of the first append_ctas CTAs of the
+// column, parts warps to a job; the other CTAs take the queries.  Every warp works out the places of the tokens
+// for itself, a token per lane.
+template <int KV, bool INTERLEAVED, int PASSES>
+__global__ void __launch_bounds__(kAppendThreads, PASSES == 1 ? 4 : 2) append_block_scaled_kernel(const AppendArgs a) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  __shared__ float tops[2][kAppendWarps];
+  const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
   const uint32_t token0 = blockIdx.x * a.tokens_per_cta;
-  TokenPlace mine{};
-  if (lane < a.tokens_per_cta) mine = place_token(a, token0 + lane);
+  const TokenPlace mine = place_token(a, token0 + lane, lane < a.tokens_per_cta, lane);
   const uint32_t D = a.head_size;
   const uint32_t heads = a.num_kv_heads;
-
+  const LaneShare lane_share(D, lane);
+  const uint32_t parts = a.warps_per_job, part = warp % parts;
+  const uint32_t jobs_at_once = kAppendWarps / parts;
+  uint32_t round = 0;
   uint32_t leaders = __ballot_sync(0xffffffffu, mine.valid && mine.leads);
+  if (blockIdx.y >= a.append_ctas) leaders = 0u;
   while (leaders != 0u) {
     const uint32_t src = __ffs(leaders) - 1u;
     leaders &= leaders - 1u;
@@ -174,59 +348,78 @@ __global__ void __launch_bounds__(512) append_block_scaled_kernel(const AppendAr
     const uint32_t block = __shfl_sync(0xffffffffu, mine.block, src);
     const uint32_t rows = __shfl_sync(0xffffffffu, mine.rows_here, src);
     const uint32_t first_row = position & (a.block_size - 1u);
-    const size_t token = token0 + src;
-    for (uint32_t job = warp; job < 2u * heads; job += warps) {
-      const bool is_v = job >= heads;
-      const uint32_t head = is_v ? job - heads : job;
-      const uint64_t stride = is_v ? a.value_stride : a.key_stride;
-      const __half *rows_src = (is_v ? a.value : a.key) + token * stride + static_cast<size_t>(head) * D;
-      uint8_t *block_rows = static_cast<uint8_t *>(is_v ? a.value_cache : a.key_cache) +
-                            (static_cast<size_t>(block) * a.block_size * heads + head) * D;
+    // a job's rows go to its warps in runs of whole row groups
+    const uint32_t run = divide_round_up(divide_round_up(rows, parts), lane_share.rows_per_pass) * lane_share.rows_per_pass;
+    const uint32_t run0 = min(rows, part * run);
+    const size_t token = token0 + src + run0;
+    const size_t block_offset = static_cast<size_t>(block) * a.block_size * heads;
+    RowJob job;
+    job.rows = min(rows - run0, run);
+    job.pitch = static_cast<size_t>(heads) * D;
+    job.rotary_dim = a.rotary_dim;
+    for (uint32_t j0 = blockIdx.y * jobs_at_once; j0 < 2u * heads; j0 += a.append_ctas * jobs_at_once, ++round) {
+      const uint32_t j = j0 + warp / parts;
+      const bool live = j < 2u * heads; // the others have nothing to do, but the CTA's warps may wait for them
+      const bool is_v = live && j >= heads;
+      const uint32_t head = !live ? 0u : is_v ? j - heads : j;
+      job.stride = is_v ? a.value_stride : a.key_stride;
+      job.src = (is_v ? a.value : a.key) + token * job.stride + static_cast<size_t>(head) * D;
+      uint8_t *block_rows = static_cast<uint8_t *>(is_v ? a.value_cache : a.key_cache) + (block_offset + head) * D;
+      job.dst = block_rows + (first_row + run0) * job.pitch;
       float *scale_at = (is_v ? a.v_scales : a.k_scales) + static_cast<size_t>(block) * heads + head;
-      append_rows<KV, INTERLEAVED>(a, rows_src, stride, !is_v && a.cos_sin != nullptr, position, block_rows, scale_at,
-                                   first_row, rows, lane);
+      float *table = tops[round & 1u]; // two rows in turn: a warp may be a round ahead of another
+      job.angles = nullptr;
+      if (is_v || a.rotary_dim == 0u) {
+        append_rows<KV, INTERLEAVED, PASSES, false>(job, lane_share, live, part, parts, first_row, block_rows, scale_at, table, lane, warp);
+      } else {
+        job.angles = a.cos_sin + static_cast<size_t>(position + run0) * a.rotary_dim;
+        append_rows<KV, INTERLEAVED, PASSES, true>(job, lane_share, live, part, parts, first_row, block_rows, scale_at, table, lane, warp);
+      }
     }
   }
 
-  if (a.query == nullptr) return;
-  uint32_t live = __ballot_sync(0xffffffffu, mine.valid);
+  if (blockIdx.y < a.append_ctas) return;
+  // queries: (token, head) pairs go round groups of head_size / 16 lanes
   const uint32_t lanes_per_head = D / 16u;
-  const uint32_t heads_per_pass = blockDim.x / lanes_per_head;
-  const uint32_t item = threadIdx.x % lanes_per_head, head0 = threadIdx.x / lanes_per_head;
-  const RotaryItem rot = rotary_item(item, a.cos_sin != nullptr ? a.rotary_dim : 0u, INTERLEAVED);
-  while (live != 0u) {
-    const uint32_t src = __ffs(live) - 1u;
-    live &= live - 1u;
-    const uint32_t position = __shfl_sync(0xffffffffu, mine.position, src);
-    const size_t token = token0 + src;
-    if (head0 >= heads_per_pass) continue;
-    float c[8], s[8];
-    if (rot.rotated) load_cos_sin(a.cos_sin + static_cast<size_t>(position) * a.rotary_dim, item, a.rotary_dim, c, s);
-    for (uint32_t head = head0; head < a.num_heads; head += heads_per_pass) {
-      const __half *row = a.query + token * a.query_stride + static_cast<size_t>(head) * D;
-      __half *dst = a.query_out + (token * a.num_heads + head) * D;
-      float x[8], y[8];
-      unpack_half8(__ldg(reinterpret_cast<const uint4 *>(row + rot.first)), x);
-      unpack_half8(__ldg(reinterpret_cast<const uint4 *>(row + rot.second)), y);
-      if (rot.rotated) rotate_item(x, y, c, s, INTERLEAVED);
-      *reinterpret_cast<uint4 *>(dst + rot.first) = pack_half8(x);
-      *reinterpret_cast<uint4 *>(dst + rot.second) = pack_half8(y);
+  const uint32_t pairs_at_once = kAppendThreads / lanes_per_head;
+  const uint32_t item = threadIdx.x % lanes_per_head, pair0 = threadIdx.x / lanes_per_head;
+  const RotaryItem rot = rotary_item(item, a.rotary_dim, INTERLEAVED);
+  const uint32_t pairs = a.tokens_per_cta * a.num_heads;
+  const uint32_t step = (gridDim.y - a.append_ctas) * pairs_at_once;
+#pragma unroll 2
+  for (uint32_t p0 = (blockIdx.y - a.append_ctas) * pairs_at_once; p0 < pairs; p0 += step) { // the same trips for all lanes: they shuffle
+    const uint32_t pair = p0 + pair0;
+    const uint32_t t = pair / a.num_heads, head = pair - t * a.num_heads;
+    const uint32_t position = __shfl_sync(0xffffffffu, mine.position, t & 31u);
+    const bool valid = __shfl_sync(0xffffffffu, mine.valid ? 1 : 0, t & 31u) != 0;
+    if (pair0 >= pairs_at_once || pair >= pairs || !valid) continue;
+    const __half *row = a.query + static_cast<size_t>(token0 + t) * a.query_stride + static_cast<size_t>(head) * D;
+    __half *dst = a.query_out + (static_cast<size_t>(token0 + t) * a.num_heads + head) * D;
+    float x[8], y[8];
+    unpack_half8(__ldg(reinterpret_cast<const uint4 *>(row + rot.first)), x);
+    unpack_half8(__ldg(reinterpret_cast<const uint4 *>(row + rot.second)), y);
+    if (rot.rotated) {
+      float c[8], s[8];
+      load_cos_sin(a.cos_sin + static_cast<size_t>(position) * a.rotary_dim, item, a.rotary_dim, c, s);
+      rotate_item(x, y, c, s, INTERLEAVED);
     }
+    *reinterpret_cast<uint4 *>(dst + rot.first) = pack_half8(x);
+    *reinterpret_cast<uint4 *>(dst + rot.second) = pack_half8(y);
   }
 }
 
-template <int KV>
-int launch_append(const AppendArgs &a, bool interleaved, cudaStream_t stream) {
+template <int KV, int PASSES>
+int launch_append(const AppendArgs &a, uint32_t query_ctas, bool interleaved, cudaStream_t stream) {
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1];
-  cfg.gridDim = dim3(divide_round_up(a.num_tokens, a.tokens_per_cta), 1, 1);
-  cfg.blockDim = dim3(32u * std::min(16u, std::max(4u, 2u * a.num_kv_heads)), 1, 1);
+  cfg.gridDim = dim3(divide_round_up(a.num_tokens, a.tokens_per_cta), a.append_ctas + query_ctas, 1);
+  cfg.blockDim = dim3(kAppendThreads, 1, 1);
   cfg.stream = stream;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  auto kernel = interleaved ? append_block_scaled_kernel<KV, true> : append_block_scaled_kernel<KV, false>;
+  auto kernel = interleaved ? append_block_scaled_kernel<KV, true, PASSES> : append_block_scaled_kernel<KV, false, PASSES>;
   PA_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a));
   return PA_OK;
 }
@@ -284,15 +477,33 @@ extern "C" PA_API int pa_append_block_scaled(const pa_block_scaled_params *p, vo
   a.block_size = p->block_size;
   a.max_blocks_per_seq = p->max_blocks_per_seq;
   a.rotary_dim = p->cos_sin != nullptr ? p->rotary_dim : 0u;
-  // as many tokens per CTA as a sequence has on average, up to a block: about one block per CTA
-  // on prompts, one token on decode steps
+  // On prompts a CTA takes 32 tokens (two blocks of 16), so that finding their places is paid for once; on decode
+  // steps one, and in between as many as a sequence has on average.
+  const uint32_t average = p->cu_tokens != nullptr ? std::max(1u, p->num_tokens / p->num_seqs) : 1u;
   uint32_t per_cta = 1;
-  if (p->cu_tokens != nullptr)
-    while (per_cta < 32u && per_cta < p->block_size && per_cta * 2u <= p->num_tokens / p->num_seqs) per_cta *= 2u;
+  while (per_cta < 32u && per_cta * 2u <= average) per_cta *= 2u;
   a.tokens_per_cta = per_cta;
+  // A few new rows per block (decode steps): one group of rows per warp, and twice the CTAs on an SM.  Otherwise four
+  // groups, and as many warps to a job as keep a block's new rows in registers.
+  const uint32_t rows = std::min(p->block_size, average);
+  const uint32_t rows_per_pass = 32u / (p->head_size / 16u);
+  const bool few = rows <= rows_per_pass;
+  uint32_t parts = 1;
+  while (parts < kAppendWarps && parts * (few ? 1u : 4u) * rows_per_pass < rows) parts *= 2u;
+  a.warps_per_job = parts;
+  // enough CTAs in a column to fill the GPU once or twice, no more than it has work for
+  const uint32_t columns = divide_round_up(p->num_tokens, per_cta);
+  const uint32_t wanted = std::max(1u, 1184u / columns);
+  a.append_ctas = std::min(wanted, divide_round_up(2u * p->num_kv_heads * parts, kAppendWarps));
+  uint32_t query_ctas = 0;
+  if (p->query != nullptr)
+    query_ctas = std::min(wanted, divide_round_up(per_cta * p->num_heads * (p->head_size / 16u), kAppendThreads));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool interleaved = p->interleaved != 0u;
-  if (p->kv_dtype == PA_KV_INT8) return launch_append<KV_I8>(a, interleaved, s);
-  if (p->kv_dtype == PA_KV_FP8_E4M3) return launch_append<KV_E4M3>(a, interleaved, s);
-  return launch_append<KV_E5M2>(a, interleaved, s);
+  auto launch = [&](auto few_rows, auto many_rows) {
+    return few ? few_rows(a, query_ctas, interleaved, s) : many_rows(a, query_ctas, interleaved, s);
+  };
+  if (p->kv_dtype == PA_KV_INT8) return launch(launch_append<KV_I8, 1>, launch_append<KV_I8, 4>);
+  if (p->kv_dtype == PA_KV_FP8_E4M3) return launch(launch_append<KV_E4M3, 1>, launch_append<KV_E4M3, 4>);
+  return launch(launch_append<KV_E5M2, 1>, launch_append<KV_E5M2, 4>);
 }

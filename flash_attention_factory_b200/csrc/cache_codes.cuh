@@ -46,6 +46,52 @@ __device__ __forceinline__ void unpack_codes(uint32_t v, float (&x)[4]) {
   x[3] = b.y;
 }
 
+// Division of many values by one scale.  q = x r with r the rounded reciprocal is off by at most two units in
+// the last place; one residual step (Markstein, "Computation of elementary functions on the IBM RISC System/6000
+// processor", 1990), q + (x - q s) r, gives the correctly rounded quotient but for rare cases of one unit,
+// so a code can differ from that of the rounded quotient only where the quotient lies within 2^-23 of
+// itself from a rounding border.  Three operations instead of a full division.  The residual needs s and 1 / s away from the ends
+// of the exponent range; other scales take the division.
+struct Divider {
+  float s, r;
+  bool plain;
+  __device__ __forceinline__ explicit Divider(float scale) {
+    s = scale;
+    r = __frcp_rn(scale);
+    plain = !(scale >= 0x1p-60f && scale <= 0x1p60f);
+  }
+  __device__ __forceinline__ float operator()(float x) const {
+    const float q = __fmul_rn(x, r);
+    return __fmaf_rn(__fmaf_rn(-q, s, x), r, q);
+  }
+};
+
+// Eight values over their scale
+__device__ __forceinline__ void divide8(float (&x)[8], const Divider &by) {
+  if (by.plain) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = __fdiv_rn(x[j], by.s);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = by(x[j]);
+  }
+}
+
+// Four finite values of at most 127.5 in size -> four codes.  Adding 1.5 * 2^23 leaves the nearest integer (ties to
+// even) in the low bits of the sum, whose low byte is the code: full-rate additions and byte
+// placements instead of float-to-integer conversions, which run at an eighth of that rate.
+template <int KV>
+__device__ __forceinline__ uint32_t pack_small_codes(float a, float b, float c, float d) {
+  if constexpr (KV == KV_I8) {
+    constexpr float kShift = 12582912.f;
+    const uint32_t ab = __byte_perm(__float_as_uint(__fadd_rn(a, kShift)), __float_as_uint(__fadd_rn(b, kShift)), 0x0040);
+    const uint32_t cd = __byte_perm(__float_as_uint(__fadd_rn(c, kShift)), __float_as_uint(__fadd_rn(d, kShift)), 0x0040);
+    return __byte_perm(ab, cd, 0x5410);
+  } else {
+    return pack_codes<KV>(a, b, c, d);
+  }
+}
+
 // Eight fp16 values of one 16-byte load as fp32
 __device__ __forceinline__ void unpack_half8(uint4 v, float (&x)[8]) {
   const __half2 *h = reinterpret_cast<const __half2 *>(&v);

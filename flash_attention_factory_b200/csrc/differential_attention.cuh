@@ -7,14 +7,13 @@
 
 namespace pa {
 
-// log2 of the partition size: the smallest power of two from 64 tokens on with which the scratch's
-// partitions cover the longest context; the last partition is open-ended, so a context beyond the
-// caller's hint is still attended to its end.
-inline uint32_t diff_partition_shift(const pa_params *p) {
-  const uint64_t longest = context_hint(p) != 0u ? context_hint(p) : context_limit(p);
-  uint32_t shift = 6;
-  while (shift < 31u && (static_cast<uint64_t>(p->max_num_partitions) << shift) < longest) ++shift;
-  return shift;
+// Partition size in tokens: the longest context spread evenly over the partitions that the scratch has
+// room for, in steps of 64.  The last partition is open-ended, so a context beyond the caller's hint is
+// still attended to its end.
+inline uint32_t diff_partition_tokens(const pa_params *p) {
+  const uint32_t longest = std::min(context_hint(p) != 0u ? context_hint(p) : context_limit(p), 1u << 30);
+  const uint32_t even = divide_round_up(std::max(longest, 1u), p->max_num_partitions);
+  return divide_round_up(even, 64u) * 64u;
 }
 
 template <int D, int KV, int TILES, int NWARPS = 4>
@@ -25,8 +24,7 @@ static int enqueue_diff(const pa_params *p, cudaStream_t stream, uint32_t hpc) {
   if (int rc = get_device_info(&dev)) return rc;
   if (dev.cc_major < 10) return fail(PA_ERR_CUDA, "this library needs an sm_100a device");
   AttnArgs args = make_attn_args<D, KV, NWARPS, TILES>(p, hpc);
-  args.partition_shift = diff_partition_shift(p);
-  args.last_partition_open = 1u;
+  args.partition_tokens = diff_partition_tokens(p);
   cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
   if (stream != nullptr && stream != cudaStreamLegacy) PA_CUDA_TRY(cudaStreamIsCapturing(stream, &capture));
   args.sched_slot = next_sched_slot(capture != cudaStreamCaptureStatusNone);

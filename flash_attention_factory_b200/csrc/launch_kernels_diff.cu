@@ -25,32 +25,36 @@ struct DiffMergeArgs {
   const uint32_t *context_lens, *seq_indices, *table_offsets;
   const float *lambdas, *norm_weight;
   uint32_t num_heads; // H
-  uint32_t max_num_partitions, partition_shift, ctx_limit, block_shift;
+  uint32_t max_num_partitions, partition_tokens, ctx_limit, block_shift;
   float norm_eps, norm_scale;
 };
 
-// One CTA of 256 threads per (sequence, head).  A thread owns 4 of the row's 2 D dims of one map and every
+// One CTA per (sequence, head), half of its threads per map.  A thread owns 4 of the row's 2 D dims and every
 // CLASSES-th partition; the first rows are requested before the weights are known, so a context of up
 // to UNROLL * CLASSES partitions costs one round trip to memory behind the context length.  Partitions
 // are added in increasing order per class, classes in increasing order: the result does not depend on
 // timing.
-template <int D>
-__global__ void __launch_bounds__(256) merge_difference_kernel(const DiffMergeArgs a) {
+constexpr uint32_t kMergeWeights = 1024; // partitions whose weights are kept in shared memory
+
+template <int D, int THREADS>
+__global__ void __launch_bounds__(THREADS) merge_difference_kernel(const DiffMergeArgs a) {
   constexpr uint32_t ROW = 2 * D;
+  constexpr uint32_t HALF_CTA = THREADS / 2;
   constexpr uint32_t LANES_PER_ROW = ROW / 4;               // 64 or 32 threads
-  constexpr uint32_t CLASSES = 128 / LANES_PER_ROW;         // 2 or 4 per map
+  constexpr uint32_t CLASSES = HALF_CTA / LANES_PER_ROW;    // partitions that a map takes at a time
   constexpr uint32_t UNROLL = 8;
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const uint32_t head = blockIdx.x;
   const uint32_t seq = (a.seq_indices != nullptr) ? __ldg(a.seq_indices + blockIdx.y) : blockIdx.y;
-  const uint32_t map = tid >> 7;
-  const uint32_t cls = (tid & 127u) / LANES_PER_ROW;
+  const uint32_t map = tid / HALF_CTA;
+  const uint32_t cls = (tid % HALF_CTA) / LANES_PER_ROW;
   const uint32_t col = (tid % LANES_PER_ROW) * 4u;
-  const size_t base = ((static_cast<size_t>(seq) * a.num_heads + head) * 2u + map) * a.max_num_partitions;
   const uint32_t NP = a.max_num_partitions;
+  const size_t base = ((static_cast<size_t>(seq) * a.num_heads + head) * 2u + map) * NP;
 
+  __shared__ float weights[2][kMergeWeights];
   __shared__ float top[2], inverse[2];
   __shared__ float part[2][CLASSES][ROW];
   __shared__ float squares[2];
@@ -63,27 +67,32 @@ __global__ void __launch_bounds__(256) merge_difference_kernel(const DiffMergeAr
                        : make_float4(0.f, 0.f, 0.f, 0.f);
   }
   const uint32_t ctx = merge_context(a.context_lens, seq, a.ctx_limit, a.table_offsets, a.block_shift);
-  const uint32_t np = min((ctx + (1u << a.partition_shift) - 1u) >> a.partition_shift, NP); // as the first kernel counts
-  // one warp per map: largest logit and total weight of its partitions
-  if ((warp & 3u) == 0u) {
+  const uint32_t np = min(divide_round_up(ctx, a.partition_tokens), NP); // as the first kernel counts
+  // one warp per map: largest logit, weights and total weight of its partitions
+  if (tid % HALF_CTA < 32u) {
     float m = neg_infinity();
     for (uint32_t p = lane; p < np; p += 32) m = fmaxf(m, a.max_logits[base + p]);
 #pragma unroll
     for (uint32_t o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float w = 0.f;
-    for (uint32_t p = lane; p < np; p += 32) w += a.exp_sums[base + p] * __expf(a.max_logits[base + p] - m);
+    float total = 0.f;
+    for (uint32_t p = lane; p < np; p += 32) {
+      const float w = a.exp_sums[base + p] * __expf(a.max_logits[base + p] - m);
+      if (p < kMergeWeights) weights[map][p] = w;
+      total += w;
+    }
 #pragma unroll
-    for (uint32_t o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+    for (uint32_t o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     if (lane == 0) {
       top[map] = m;
-      inverse[map] = (w > 0.f) ? 1.f / w : 0.f;
+      inverse[map] = (total > 0.f) ? 1.f / total : 0.f;
     }
   }
   __syncthreads();
   const float m = top[map], inv = inverse[map];
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
   auto add = [&](float4 v, uint32_t p) {
-    const float w = a.exp_sums[base + p] * __expf(a.max_logits[base + p] - m) * inv;
+    const float w =
+        ((p < kMergeWeights) ? weights[map][p] : a.exp_sums[base + p] * __expf(a.max_logits[base + p] - m)) * inv;
     sum.x += w * v.x;
     sum.y += w * v.y;
     sum.z += w * v.z;
@@ -163,7 +172,7 @@ int enqueue_difference(const pa_diff_params *d, cudaStream_t stream) {
   a.norm_weight = d->norm_weight;
   a.num_heads = p->num_heads / 2u;
   a.max_num_partitions = p->max_num_partitions;
-  a.partition_shift = diff_partition_shift(p);
+  a.partition_tokens = diff_partition_tokens(p);
   a.ctx_limit = context_limit(p);
   a.block_shift = log2_pow2(p->block_size);
   a.norm_eps = d->norm_eps;
@@ -171,13 +180,21 @@ int enqueue_difference(const pa_diff_params *d, cudaStream_t stream) {
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1];
   cfg.gridDim = dim3(a.num_heads, p->num_seqs, 1);
-  cfg.blockDim = dim3(256, 1, 1);
   cfg.stream = stream;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  PA_CUDA_TRY(cudaLaunchKernelEx(&cfg, merge_difference_kernel<D>, a));
+  // Many partitions of few rows: more threads take more of them at a time (64 rows of 74 partitions: 10 us
+  // instead of 15).  With more rows than the GPU holds CTAs of 1024 threads the small ones win (768 rows of 48:
+  // 11 us instead of 25).
+  if (p->max_num_partitions > 32u && static_cast<uint64_t>(a.num_heads) * p->num_seqs <= 296u) {
+    cfg.blockDim = dim3(1024, 1, 1);
+    PA_CUDA_TRY(cudaLaunchKernelEx(&cfg, merge_difference_kernel<D, 1024>, a));
+  } else {
+    cfg.blockDim = dim3(256, 1, 1);
+    PA_CUDA_TRY(cudaLaunchKernelEx(&cfg, merge_difference_kernel<D, 256>, a));
+  }
   return PA_OK;
 }
 
@@ -208,17 +225,29 @@ PA_TIMELINE_ACCESSOR(pa_debug_timeline_diff)
 PA_BOUNDS_ACCESSOR(pa_debug_bounds_diff)
 
 extern "C" PA_API uint32_t pa_diff_num_partitions(uint32_t num_seqs, uint32_t num_kv_heads, uint32_t head_size,
-                                                  uint32_t max_context_len) {
+                                                  uint32_t max_context_len, int32_t kv_dtype) {
   using namespace pa;
   if ((head_size != 128 && head_size != 64) || num_kv_heads == 0 || num_kv_heads % 2u != 0u) return 0;
+  if (kv_dtype != PA_KV_F16 && kv_dtype != PA_KV_FP8_E5M2 && kv_dtype != PA_KV_FP8_E4M3 && kv_dtype != PA_KV_INT8) return 0;
   if (max_context_len == 0 || num_seqs == 0) return 1;
-  // 512 tokens: a partition of 4 heads of 128 bytes then is 512 KB, an item the ring streams without a gap.
-  // Shorter ones, down to 64 tokens, while there are fewer items than the 296 CTAs that are resident on 148 SMs.
-  const uint64_t units = static_cast<uint64_t>(num_seqs) * (num_kv_heads / (num_kv_heads % 4u == 0u ? 4u : 2u));
-  uint32_t size = 512;
-  while (size > 64u && units * divide_round_up(max_context_len, size) < 296u) size /= 2u;
-  // the kernel's index arithmetic holds 65535 partitions of a sequence
-  return std::min(65535u, divide_round_up(max_context_len, size));
+  // An item (a partition of the 4 or 2 heads of a CTA) of 512 KB: smaller ones show the cost of an item, larger
+  // ones leave CTAs idle at the end of a ragged batch (48 sequences up to 8192 tokens, fp16, 8 KV heads of 128:
+  // 127 us with 256 tokens, 138 with 512, 167 with 1024, 149 with 171).
+  const uint32_t hpc = num_kv_heads % 4u == 0u ? 4u : 2u;
+  const uint32_t token_bytes = hpc * head_size * 2u * (kv_dtype == PA_KV_F16 ? 2u : 1u);
+  const uint32_t usual = divide_round_up(max_context_len, (512u << 10) / token_bytes);
+  const uint64_t units = static_cast<uint64_t>(num_seqs) * (num_kv_heads / hpc);
+  const uint64_t items = units * usual, slots = 296u; // CTAs resident on 148 SMs
+  uint64_t parts = usual;
+  // With few items the last round of CTAs counts: the contexts are cut so that whole rounds are full, in
+  // partitions of at least 64 tokens (2 sequences of 65536 tokens, e4m3: 58 us with 74 partitions, one item for
+  // every CTA, 68 us with 128, 81 us with 111).
+  if (items < 4u * slots) {
+    const uint64_t rounds = std::max<uint64_t>(1u, items / slots);
+    parts = std::max<uint64_t>(1u, rounds * slots / units);
+    parts = std::min<uint64_t>(parts, divide_round_up(max_context_len, 64u));
+  }
+  return static_cast<uint32_t>(std::min<uint64_t>(65535u, parts)); // the kernel's index arithmetic
 }
 
 extern "C" PA_API int launch_kernels_diff(const pa_diff_params *p, void *stream, float *us_out) {

@@ -166,9 +166,9 @@ struct AttnArgs {
   // context of a (sequence, head group), its normalised result goes straight to `out`, and the
   // scratch tensors are neither read nor written (they may be null)
   uint32_t whole_context_items;
-  // split mode: the last partition that the scratch has room for runs to the end of the context,
-  // whatever its length (differential attention, whose partition size follows from the scratch)
-  uint32_t last_partition_open;
+  // differential attention: the partition size in tokens, any multiple of 64, in the place of
+  // partition_shift; the last partition that the scratch has room for is open-ended.  0 otherwise.
+  uint32_t partition_tokens;
   // max_blocks_per_seq * block_size (saturated to 32 bits): a context length beyond it is cut
   // to it, so no block-table read leaves the sequence's row whatever context_lens holds
   uint32_t ctx_limit;
@@ -208,9 +208,10 @@ struct SmemLayout {
   static constexpr uint32_t STAGE_BYTES = 2 * KV_TILE;
   static constexpr uint32_t RING_BYTES = NSTAGES * STAGE_BYTES;
   static_assert(NW == 4 || NW == 8, "warp <-> (head, token slice) mapping: 4 warps, or 8 with one head per warp");
-  // split mode, fewer than 4 heads per CTA: two O[8][VH * D] buffers filled in a fixed order
+  // split mode, fewer than 4 heads per CTA: two O[8][D] buffers filled in a fixed order (one V head
+  // after the other where there are two: buffers for both would leave room for one CTA per SM only)
   static constexpr uint32_t MERGE_OFFSET = RING_BYTES;
-  static constexpr uint32_t MERGE_BYTES = (NWARPS == 8) ? 0 : 2 * 8 * VH * D * 4; // the wide CTA never merges
+  static constexpr uint32_t MERGE_BYTES = (NWARPS == 8) ? 0 : 2 * 8 * D * 4; // the wide CTA never merges
   // per-warp (reference max, true max, sum) of the 8 query columns, double-buffered by item parity
   static constexpr uint32_t WARP_STATS_OFFSET = MERGE_OFFSET + MERGE_BYTES;
   static constexpr uint32_t WARP_STATS_FLOATS = 3 * NW * 8;
@@ -296,6 +297,7 @@ struct SplitCursor {
   // launch, an empty one included, is exactly one (its output row has to be written)
   static __device__ __forceinline__ uint32_t parts_of(const AttnArgs &args, uint32_t ctx) {
     if (args.whole_context_items != 0u) return 1u;
+    if (args.partition_tokens != 0u) return min(divide_round_up(ctx, args.partition_tokens), args.max_num_partitions);
     const uint32_t psize = 1u << args.partition_shift;
     return min((ctx + psize - 1u) >> args.partition_shift, args.max_num_partitions);
   }
@@ -367,9 +369,13 @@ struct SplitCursor {
       it.tok_begin = 0u;
       it.tok_end = ctx;
     } else {
-      it.tok_begin = it.partition << args.partition_shift;
-      it.tok_end = min(ctx, it.tok_begin + (1u << args.partition_shift));
-      if (args.last_partition_open != 0u && it.partition + 1u == args.max_num_partitions) it.tok_end = ctx;
+      if (args.partition_tokens != 0u) {
+        it.tok_begin = it.partition * args.partition_tokens;
+        it.tok_end = (it.partition + 1u == args.max_num_partitions) ? ctx : min(ctx, it.tok_begin + args.partition_tokens);
+      } else {
+        it.tok_begin = it.partition << args.partition_shift;
+        it.tok_end = min(ctx, it.tok_begin + (1u << args.partition_shift));
+      }
     }
     it.ctx = ctx;
     it.table_off = __shfl_sync(0xffffffffu, lane_off, owner);
@@ -537,6 +543,12 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
   constexpr uint32_t NSTAGES = L::NSTAGES;
   constexpr uint32_t KSTEPS = D / 16; // MMA k-steps of QK^T == accumulator tiles of PV
   constexpr uint32_t NCONS = NW * 32; // consumer threads
+  // Integer K tiles go into the MMA as they are, as fp16 subnormals: a code c plus 128 in the low byte
+  // of a half is (c + 128) * 2^-24.  The accumulator starts at -128 * 2^-24 * sum_d q_d, so a score comes
+  // out as 2^-24 q.c, three operations per four codes instead of five; the offset is of the size of the
+  // codes, so the fp32 sum over at most 128 dims keeps its precision.  (V codes are converted in full: there the offset
+  // would grow with the number of tokens.)
+  constexpr float kKeyUnit = (KV == KV_I8) ? 16777216.f : 1.f; // what a raw score is multiplied by
 
   extern __shared__ uint8_t smem_raw[];
   // 1024-byte alignment of the ring makes the TMA swizzle a function of (row, chunk).
@@ -581,7 +593,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
   // the wait for the previous kernel of the stream
   if (threadIdx.x == 0) {
     for (uint32_t s = 0; s < NSTAGES; ++s) {
-      mbar_init(&full_bar[s], 1);   // one arrive.expect_tx by the producer
+      // one arrive.expect_tx by the producer; with per-block scales also one arrival of every producer
+      // lane behind the scales it copies
+      mbar_init(&full_bar[s], block_scales ? 33u : 1u);
       mbar_init(&empty_bar[s], NW); // one arrive per consumer warp
     }
     for (uint32_t s = 0; s < 2; ++s) {
@@ -759,25 +773,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
         const int32_t y = static_cast<int32_t>((block_id << args.block_shift) + (tok & row_mask));
         const uint32_t chunks_in_batch = min(chunks_per_batch, total_chunks - chunk0);
         const uint32_t stages_in_batch = divide_round_up(chunks_in_batch, chunks_per_stage);
-        // per-block scales of this lane's (block, head): requested now, written beside the stage
-        // before it is armed; in steady state the wait for a free stage hides the latency
-        float2 lane_scales = make_float2(1.f, 1.f);
-        if (block_scales && valid) {
-          // a block id beyond the cache reads zeros through the descriptor; its scales come from the last block
-          const size_t si = static_cast<size_t>(min(block_id, args.num_blocks - 1u)) * args.num_kv_heads +
-                            cur.head_base + lane_head;
-          lane_scales = make_float2(__ldg(args.k_scale_per_block + si), __ldg(args.v_scale_per_block + si));
-        }
         for (uint32_t sb = 0; sb < stages_in_batch; ++sb) {
           if (lane == 0) alive = mbar_wait_bounded(&empty_bar[slot], phase ^ 1u, abort_flag);
           alive = __shfl_sync(0xffffffffu, alive ? 1 : 0, 0) != 0;
           if (!alive) break;
-          if (block_scales) {
-            // the stage is free: its scale slots may be overwritten; the arming below releases them
-            if (valid && lane_chunk / chunks_per_stage == sb)
-              stage_scales[slot * L::SCALE_SLOTS + (lane_chunk % chunks_per_stage) * hpc + lane_head] = lane_scales;
-            __syncwarp();
-          }
           if (lane == 0) {
             const uint32_t chunks_here = min(chunks_per_stage, chunks_in_batch - sb * chunks_per_stage);
             mbar_arrive_expect_tx(&full_bar[slot], chunks_here * hpc * box_bytes * 2u);
@@ -799,6 +798,21 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
               tma_load_3d(dst, &tmap_k, &full_bar[slot], x, y, head_coord, kv_policy);
               tma_load_3d(dst + L::KV_TILE, &tmap_v, &full_bar[slot], x, y, head_coord, kv_policy);
             }
+          }
+          if (block_scales) {
+            // The scales of the stage's (block, head) pairs travel like its tiles: 4-byte asynchronous
+            // copies into the slots beside the stage, whose barrier every lane arrives on when its own have
+            // landed.  (Fetching them into registers before the stage is armed held every batch of copies
+            // back by a trip to memory: 128 sequences up to 8192 tokens of int8, 169 us instead of 158.)
+            if (valid && lane_chunk / chunks_per_stage == sb) {
+              // a block id beyond the cache reads zeros through the descriptor; its scales come from the last block
+              const size_t si = static_cast<size_t>(min(block_id, args.num_blocks - 1u)) * args.num_kv_heads +
+                                cur.head_base + lane_head;
+              float2 *dst = stage_scales + slot * L::SCALE_SLOTS + (lane_chunk % chunks_per_stage) * hpc + lane_head;
+              copy_async_4(&dst->x, args.k_scale_per_block + si);
+              copy_async_4(&dst->y, args.v_scale_per_block + si);
+            }
+            mbar_arrive_after_copies(&full_bar[slot]);
           }
           if (++slot == NSTAGES) {
             slot = 0;
@@ -844,8 +858,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
 
     // S^T tile of 16 tokens: K (A operand) from shared memory at k_addr, Q from registers;
     // two accumulation chains shorten the dependency
+    float q_bias[2] = {0.f, 0.f}; // int8: where the scores of query columns 2*t4, 2*t4+1 start
     auto score_tile = [&](uint32_t k_addr, const uint32_t (&q)[KSTEPS][2], float (&c)[4]) {
-      float s_a[4] = {0.f, 0.f, 0.f, 0.f};
+      float s_a[4] = {q_bias[0], q_bias[1], q_bias[0], q_bias[1]};
       float s_b[4] = {0.f, 0.f, 0.f, 0.f};
       if constexpr (KV == KV_F16) {
 #pragma unroll
@@ -862,11 +877,11 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
           uint32_t r[4];
           ldmatrix_x4(r, k_addr ^ (qq << 5));
           uint32_t a[4];
-          fp8x4_to_half2x2<KV>(r[0], a[0], a[2]);
-          fp8x4_to_half2x2<KV>(r[1], a[1], a[3]);
+          key_codes_to_half2x2<KV>(r[0], a[0], a[2]);
+          key_codes_to_half2x2<KV>(r[1], a[1], a[3]);
           mma_m16n8k16(s_a, a, q[2 * qq][0], q[2 * qq][1]);
-          fp8x4_to_half2x2<KV>(r[2], a[0], a[2]);
-          fp8x4_to_half2x2<KV>(r[3], a[1], a[3]);
+          key_codes_to_half2x2<KV>(r[2], a[0], a[2]);
+          key_codes_to_half2x2<KV>(r[3], a[1], a[3]);
           mma_m16n8k16(s_b, a, q[2 * qq + 1][0], q[2 * qq + 1][1]);
         }
       }
@@ -879,8 +894,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
     // those of score_tile, hence the same bits.
     auto score_tile_pair = [&](uint32_t ka_addr, uint32_t kb_addr, const uint32_t (&q)[KSTEPS][2],
                                float (&ca)[4], float (&cb)[4]) {
-      float a0[4] = {0.f, 0.f, 0.f, 0.f}, a1[4] = {0.f, 0.f, 0.f, 0.f};
-      float b0[4] = {0.f, 0.f, 0.f, 0.f}, b1[4] = {0.f, 0.f, 0.f, 0.f};
+      float a0[4] = {q_bias[0], q_bias[1], q_bias[0], q_bias[1]}, a1[4] = {0.f, 0.f, 0.f, 0.f};
+      float b0[4] = {q_bias[0], q_bias[1], q_bias[0], q_bias[1]}, b1[4] = {0.f, 0.f, 0.f, 0.f};
       if constexpr (KV == KV_F16) {
 #pragma unroll
         for (uint32_t ks = 0; ks < KSTEPS; ++ks) {
@@ -902,17 +917,17 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
           uint32_t ra[4], rb[4], fa[4], fb[4];
           ldmatrix_x4(ra, ka_addr ^ (qq << 5));
           ldmatrix_x4(rb, kb_addr ^ (qq << 5));
-          fp8x4_to_half2x2<KV>(ra[0], fa[0], fa[2]);
-          fp8x4_to_half2x2<KV>(ra[1], fa[1], fa[3]);
+          key_codes_to_half2x2<KV>(ra[0], fa[0], fa[2]);
+          key_codes_to_half2x2<KV>(ra[1], fa[1], fa[3]);
           mma_m16n8k16(a0, fa, q[2 * qq][0], q[2 * qq][1]);
-          fp8x4_to_half2x2<KV>(rb[0], fb[0], fb[2]);
-          fp8x4_to_half2x2<KV>(rb[1], fb[1], fb[3]);
+          key_codes_to_half2x2<KV>(rb[0], fb[0], fb[2]);
+          key_codes_to_half2x2<KV>(rb[1], fb[1], fb[3]);
           mma_m16n8k16(b0, fb, q[2 * qq][0], q[2 * qq][1]);
-          fp8x4_to_half2x2<KV>(ra[2], fa[0], fa[2]);
-          fp8x4_to_half2x2<KV>(ra[3], fa[1], fa[3]);
+          key_codes_to_half2x2<KV>(ra[2], fa[0], fa[2]);
+          key_codes_to_half2x2<KV>(ra[3], fa[1], fa[3]);
           mma_m16n8k16(a1, fa, q[2 * qq + 1][0], q[2 * qq + 1][1]);
-          fp8x4_to_half2x2<KV>(rb[2], fb[0], fb[2]);
-          fp8x4_to_half2x2<KV>(rb[3], fb[1], fb[3]);
+          key_codes_to_half2x2<KV>(rb[2], fb[0], fb[2]);
+          key_codes_to_half2x2<KV>(rb[3], fb[1], fb[3]);
           mma_m16n8k16(b1, fb, q[2 * qq + 1][0], q[2 * qq + 1][1]);
         }
       }
@@ -1049,9 +1064,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
     };
     // K scale (log2-domain softmax scale) and V scales of the tile that starts at `row` of a stage.
     // A zero scale (a block of zeros) keeps a tiny positive softmax scale, so that -inf stays -inf.
+    const uint32_t box_shift = 31u - __clz(args.rows_per_box); // a power of two, like both it is the smaller of
     auto tile_scales = [&](uint32_t stage_slot, uint32_t row, float &k_scale, float (&v)[VH]) {
-      const float2 *s = stage_scales + stage_slot * L::SCALE_SLOTS + (row / args.rows_per_box) * hpc;
-      k_scale = fmaxf(args.sm_scale_log2 * s[my_head].x, 1e-30f);
+      const float2 *s = stage_scales + stage_slot * L::SCALE_SLOTS + (row >> box_shift) * hpc;
+      k_scale = fmaxf(args.sm_scale_log2 * kKeyUnit * s[my_head].x, 1e-30f);
 #pragma unroll
       for (uint32_t vh = 0; vh < VH; ++vh) v[vh] = s[v_head0 + vh].y;
     };
@@ -1062,9 +1078,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
       nxt.valid = false;
       const uint32_t kv_head = cur.head_base + my_head;
       // softmax scale (log2 domain) and output scale of this warp's KV head
-      const float scale = (args.k_scale_per_head != nullptr)
-                              ? args.sm_scale_log2 * __ldg(args.k_scale_per_head + kv_head)
-                              : args.scale_log2;
+      const float scale = ((args.k_scale_per_head != nullptr)
+                               ? args.sm_scale_log2 * __ldg(args.k_scale_per_head + kv_head)
+                               : args.scale_log2) *
+                          kKeyUnit;
       float out_scale[VH];
 #pragma unroll
       for (uint32_t vh = 0; vh < VH; ++vh)
@@ -1090,6 +1107,22 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
         for (uint32_t i = 0; i < KSTEPS; ++i) acc[vh][i][0] = acc[vh][i][1] = acc[vh][i][2] = acc[vh][i][3] = 0.f;
       }
       v_ref = v_inv = 0.f;
+      if constexpr (KV == KV_I8) {
+        float sum = 0.f; // of this lane's quarter of column gid
+#pragma unroll
+        for (uint32_t ks = 0; ks < KSTEPS; ++ks) {
+#pragma unroll
+          for (uint32_t j = 0; j < 2; ++j) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&qf[ks][j]));
+            sum += f.x + f.y;
+          }
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+        for (uint32_t j = 0; j < 2; ++j)
+          q_bias[j] = __shfl_sync(0xffffffffu, sum, (2 * t4 + j) * 4u) * (-128.f / 16777216.f);
+      }
       // The sink is one extra logit with a zero value vector, attached to the first tokens
       // of the context only (reference paged_attention_kernel_loop.hpp:387-401).
       if (args.sinks != nullptr && my_slice == 0 && cur.tok_begin == 0) {
@@ -1455,89 +1488,87 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
           // hpc = 2: buffer = head, slice 0 stores and slice 1 adds
           const uint32_t buf_id = (hpc == 1) ? (my_slice & 1u) : my_head;
           const uint32_t round = (hpc == 1) ? (my_slice >> 1) : my_slice;
-          constexpr uint32_t ROW = VH * D; // floats of a buffer row
-          float *buf = merge_buf + buf_id * (8 * ROW);
-          if (round == 0) {
+          float *buf = merge_buf + buf_id * (8 * D);
+          // one V head at a time
 #pragma unroll
-            for (uint32_t vh = 0; vh < VH; ++vh) {
-#pragma unroll
-              for (uint32_t i = 0; i < KSTEPS; ++i) {
-#pragma unroll
-                for (uint32_t h = 0; h < 2; ++h) {
-                  const uint32_t d = vh * D + acc_dim_index<KV>(i, h, gid);
-                  buf[(2 * t4) * ROW + d] = acc[vh][i][2 * h] * f[0];
-                  buf[(2 * t4 + 1) * ROW + d] = acc[vh][i][2 * h + 1] * f[1];
-                }
-              }
-            }
-          }
-          named_barrier_sync(1, NCONS);
-          if (round == 1) {
-#pragma unroll
-            for (uint32_t vh = 0; vh < VH; ++vh) {
+          for (uint32_t vh = 0; vh < VH; ++vh) {
+            if (vh != 0) named_barrier_sync(1, NCONS); // the buffers have been read
+            if (round == 0) {
 #pragma unroll
               for (uint32_t i = 0; i < KSTEPS; ++i) {
 #pragma unroll
                 for (uint32_t h = 0; h < 2; ++h) {
-                  const uint32_t d = vh * D + acc_dim_index<KV>(i, h, gid);
-                  buf[(2 * t4) * ROW + d] += acc[vh][i][2 * h] * f[0];
-                  buf[(2 * t4 + 1) * ROW + d] += acc[vh][i][2 * h + 1] * f[1];
+                  const uint32_t d = acc_dim_index<KV>(i, h, gid);
+                  buf[(2 * t4) * D + d] = acc[vh][i][2 * h] * f[0];
+                  buf[(2 * t4 + 1) * D + d] = acc[vh][i][2 * h + 1] * f[1];
                 }
               }
             }
-          }
-          named_barrier_sync(1, NCONS);
-          // write out: thread -> (head, query column g, 8 consecutive dims)
-          constexpr uint32_t THREADS_PER_ROW = ROW / 8;
-          for (uint32_t idx = ctid; idx < hpc * 8 * THREADS_PER_ROW; idx += NCONS) {
-            const uint32_t hh = idx / (8 * THREADS_PER_ROW);
-            const uint32_t g = (idx / THREADS_PER_ROW) % 8;
-            const uint32_t d0 = (idx % THREADS_PER_ROW) * 8;
-            const uint32_t wb = hh * slices;
-            float mr_all = neg_infinity(), mt_all = neg_infinity();
-            for (uint32_t w = wb; w < wb + slices; ++w) {
-              mr_all = fmaxf(mr_all, st_ref[w * 8 + g]);
-              mt_all = fmaxf(mt_all, st_true[w * 8 + g]);
-            }
-            float l_all = 0.f;
-            for (uint32_t w = wb; w < wb + slices; ++w) {
-              const float mw = st_ref[w * 8 + g];
-              l_all += (mw == neg_infinity()) ? 0.f : fast_exp2(mw - mr_all) * st_sum[w * 8 + g];
-            }
-            const float *b0 = merge_buf + ((hpc == 1) ? 0u : hh) * (8 * ROW) + g * ROW + d0;
-            float4 lo = *reinterpret_cast<const float4 *>(b0);
-            float4 hi = *reinterpret_cast<const float4 *>(b0 + 4);
-            if (hpc == 1) {
-              const float4 lo1 = *reinterpret_cast<const float4 *>(b0 + 8 * ROW);
-              const float4 hi1 = *reinterpret_cast<const float4 *>(b0 + 8 * ROW + 4);
-              lo.x += lo1.x; lo.y += lo1.y; lo.z += lo1.z; lo.w += lo1.w;
-              hi.x += hi1.x; hi.y += hi1.y; hi.z += hi1.z; hi.w += hi1.w;
-            }
-            if (g < G && ok) {
-              const size_t head =
-                  static_cast<size_t>(cur.seq) * args.num_heads + query_head_of<VH>(cur.head_base + hh, G, g);
-              const size_t pidx = head * args.max_num_partitions + cur.partition;
-              const uint32_t v_head = cur.head_base + ((VH == 1) ? hh : (hh & ~1u) + d0 / D); // of these dims
-              const float head_scale =
-                  (args.v_scale_per_head != nullptr) ? __ldg(args.v_scale_per_head + v_head) : args.out_scale;
-              const float inv = (l_all > 0.f) ? (head_scale / l_all) : 0.f;
-              const bool whole = args.whole_context_items != 0u;
-              if constexpr (VH == 1) {
-                uint4 packed;
-                packed.x = pack_half2(lo.x * inv, lo.y * inv);
-                packed.y = pack_half2(lo.z * inv, lo.w * inv);
-                packed.z = pack_half2(hi.x * inv, hi.y * inv);
-                packed.w = pack_half2(hi.z * inv, hi.w * inv);
-                __half *dst = whole ? args.out + head * D : args.tmp_out + pidx * D;
-                *reinterpret_cast<uint4 *>(dst + d0) = packed;
-              } else {
-                float4 *dst = reinterpret_cast<float4 *>(reinterpret_cast<float *>(args.tmp_out) + pidx * ROW + d0);
-                dst[0] = make_float4(lo.x * inv, lo.y * inv, lo.z * inv, lo.w * inv);
-                dst[1] = make_float4(hi.x * inv, hi.y * inv, hi.z * inv, hi.w * inv);
+            named_barrier_sync(1, NCONS);
+            if (round == 1) {
+#pragma unroll
+              for (uint32_t i = 0; i < KSTEPS; ++i) {
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h) {
+                  const uint32_t d = acc_dim_index<KV>(i, h, gid);
+                  buf[(2 * t4) * D + d] += acc[vh][i][2 * h] * f[0];
+                  buf[(2 * t4 + 1) * D + d] += acc[vh][i][2 * h + 1] * f[1];
+                }
               }
-              if (d0 == 0 && !whole) {
-                args.max_logits[pidx] = mt_all * kLn2;
-                args.exp_sums[pidx] = l_all * fast_exp2(mr_all - mt_all);
+            }
+            named_barrier_sync(1, NCONS);
+            // write out: thread -> (head, query column g, 8 consecutive dims)
+            constexpr uint32_t THREADS_PER_ROW = D / 8;
+            for (uint32_t idx = ctid; idx < hpc * 8 * THREADS_PER_ROW; idx += NCONS) {
+              const uint32_t hh = idx / (8 * THREADS_PER_ROW);
+              const uint32_t g = (idx / THREADS_PER_ROW) % 8;
+              const uint32_t d0 = (idx % THREADS_PER_ROW) * 8;
+              const uint32_t wb = hh * slices;
+              float mr_all = neg_infinity(), mt_all = neg_infinity();
+              for (uint32_t w = wb; w < wb + slices; ++w) {
+                mr_all = fmaxf(mr_all, st_ref[w * 8 + g]);
+                mt_all = fmaxf(mt_all, st_true[w * 8 + g]);
+              }
+              float l_all = 0.f;
+              for (uint32_t w = wb; w < wb + slices; ++w) {
+                const float mw = st_ref[w * 8 + g];
+                l_all += (mw == neg_infinity()) ? 0.f : fast_exp2(mw - mr_all) * st_sum[w * 8 + g];
+              }
+              const float *b0 = merge_buf + ((hpc == 1) ? 0u : hh) * (8 * D) + g * D + d0;
+              float4 lo = *reinterpret_cast<const float4 *>(b0);
+              float4 hi = *reinterpret_cast<const float4 *>(b0 + 4);
+              if (hpc == 1) {
+                const float4 lo1 = *reinterpret_cast<const float4 *>(b0 + 8 * D);
+                const float4 hi1 = *reinterpret_cast<const float4 *>(b0 + 8 * D + 4);
+                lo.x += lo1.x; lo.y += lo1.y; lo.z += lo1.z; lo.w += lo1.w;
+                hi.x += hi1.x; hi.y += hi1.y; hi.z += hi1.z; hi.w += hi1.w;
+              }
+              if (g < G && ok) {
+                const size_t head =
+                    static_cast<size_t>(cur.seq) * args.num_heads + query_head_of<VH>(cur.head_base + hh, G, g);
+                const size_t pidx = head * args.max_num_partitions + cur.partition;
+                const uint32_t v_head = cur.head_base + ((VH == 1) ? hh : (hh & ~1u) + vh); // of these dims
+                const float head_scale =
+                    (args.v_scale_per_head != nullptr) ? __ldg(args.v_scale_per_head + v_head) : args.out_scale;
+                const float inv = (l_all > 0.f) ? (head_scale / l_all) : 0.f;
+                const bool whole = args.whole_context_items != 0u;
+                if constexpr (VH == 1) {
+                  uint4 packed;
+                  packed.x = pack_half2(lo.x * inv, lo.y * inv);
+                  packed.y = pack_half2(lo.z * inv, lo.w * inv);
+                  packed.z = pack_half2(hi.x * inv, hi.y * inv);
+                  packed.w = pack_half2(hi.z * inv, hi.w * inv);
+                  __half *dst = whole ? args.out + head * D : args.tmp_out + pidx * D;
+                  *reinterpret_cast<uint4 *>(dst + d0) = packed;
+                } else {
+                  float4 *dst = reinterpret_cast<float4 *>(reinterpret_cast<float *>(args.tmp_out) + pidx * (VH * D) + vh * D + d0);
+                  dst[0] = make_float4(lo.x * inv, lo.y * inv, lo.z * inv, lo.w * inv);
+                  dst[1] = make_float4(hi.x * inv, hi.y * inv, hi.z * inv, hi.w * inv);
+                }
+                if (d0 == 0 && vh == 0 && !whole) {
+                  args.max_logits[pidx] = mt_all * kLn2;
+                  args.exp_sums[pidx] = l_all * fast_exp2(mr_all - mt_all);
+                }
               }
             }
           }

@@ -13,6 +13,7 @@ namespace pa {
 namespace {
 
 constexpr uint32_t kRopeThreads = 128;
+constexpr uint32_t kRopeBatch = 3; // heads whose rows a thread requests together
 
 struct RopeArgs {
   const __half *query, *key, *value;
@@ -27,13 +28,12 @@ struct RopeArgs {
 };
 
 template <int KV>
-__device__ __forceinline__ void store_piece(void *row, uint32_t elem, const float (&x)[8], float scale) {
+__device__ __forceinline__ void store_piece(void *row, uint32_t elem, const float (&x)[8], const Divider &by) {
   if constexpr (KV == KV_F16) {
     *reinterpret_cast<uint4 *>(static_cast<__half *>(row) + elem) = pack_half8(x);
   } else {
-    float q[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) q[j] = __fdiv_rn(x[j], scale);
+    float q[8] = {x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]};
+    divide8(q, by);
     *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(row) + elem) =
         make_uint2(pack_codes<KV>(q[0], q[1], q[2], q[3]), pack_codes<KV>(q[4], q[5], q[6], q[7]));
   }
@@ -52,8 +52,6 @@ __global__ void __launch_bounds__(kRopeThreads) rope_and_cache_kernel(const Rope
   const uint32_t token = blockIdx.x;
   const int64_t slot = __ldg(a.slots + token);
   const int64_t position = __ldg(a.positions + token);
-  if (slot < 0 || static_cast<uint64_t>(slot) >= a.num_slots) return; // padding token / out of range
-  if (position < 0 || static_cast<uint64_t>(position) >= a.max_position) return;
   const uint32_t D = a.head_size;
   const uint32_t lanes_per_head = D / 16u;
   const uint32_t heads_per_pass = kRopeThreads / lanes_per_head;
@@ -61,47 +59,67 @@ __global__ void __launch_bounds__(kRopeThreads) rope_and_cache_kernel(const Rope
   const uint32_t head0 = threadIdx.x / lanes_per_head;
   if (head0 >= heads_per_pass) return;
   const RotaryItem rot = rotary_item(item, a.rotary_dim, INTERLEAVED);
+  const uint32_t rotated_heads = a.num_heads + a.num_kv_heads;
+  const uint32_t total = rotated_heads + a.num_kv_heads;
+  // the rows of kRopeBatch heads at a time; the first ones are on their way before the slot and the position
+  // are known (the rows of a skipped token are read in vain)
+  uint4 raw[kRopeBatch][2];
+  auto load = [&](uint32_t first) {
+#pragma unroll
+    for (uint32_t i = 0; i < kRopeBatch; ++i) {
+      const uint32_t head = first + i * heads_per_pass;
+      if (head < total) {
+        const bool is_v = head >= rotated_heads;
+        const __half *src =
+            (head < a.num_heads) ? a.query + static_cast<size_t>(token) * a.query_stride + static_cast<size_t>(head) * D
+            : is_v ? a.value + static_cast<size_t>(token) * a.value_stride + static_cast<size_t>(head - rotated_heads) * D
+                   : a.key + static_cast<size_t>(token) * a.key_stride + static_cast<size_t>(head - a.num_heads) * D;
+        raw[i][0] = __ldg(reinterpret_cast<const uint4 *>(src + rot.first));
+        raw[i][1] = __ldg(reinterpret_cast<const uint4 *>(src + rot.second));
+      }
+    }
+  };
+  load(head0);
+  if (slot < 0 || static_cast<uint64_t>(slot) >= a.num_slots) return; // padding token / out of range
+  if (position < 0 || static_cast<uint64_t>(position) >= a.max_position) return;
   float c[8], s[8];
   if (rot.rotated) load_cos_sin(a.cos_sin + static_cast<size_t>(position) * a.rotary_dim, item, a.rotary_dim, c, s);
 
-  const __half *q = a.query + static_cast<size_t>(token) * a.query_stride;
-  const __half *k = a.key + static_cast<size_t>(token) * a.key_stride;
-  const __half *v = a.value + static_cast<size_t>(token) * a.value_stride;
   __half *qo = a.query_out + static_cast<size_t>(token) * a.num_heads * D;
   constexpr uint32_t ELT = (KV == KV_F16) ? 2u : 1u;
   const size_t row_bytes = static_cast<size_t>(a.num_kv_heads) * D * ELT;
   uint8_t *kc = static_cast<uint8_t *>(a.key_cache) + static_cast<size_t>(slot) * row_bytes;
   uint8_t *vc = static_cast<uint8_t *>(a.value_cache) + static_cast<size_t>(slot) * row_bytes;
-  const uint32_t rotated_heads = a.num_heads + a.num_kv_heads;
-  const uint32_t total = rotated_heads + a.num_kv_heads;
-#pragma unroll 2
-  for (uint32_t head = head0; head < total; head += heads_per_pass) {
-    const bool is_v = head >= rotated_heads;
-    const bool is_q = head < a.num_heads;
-    const uint32_t kv_head = is_v ? head - rotated_heads : head - a.num_heads; // of K and V rows
-    const __half *src = is_q ? q + static_cast<size_t>(head) * D : (is_v ? v : k) + static_cast<size_t>(kv_head) * D;
-    // V rows take the same two pieces; they are only not rotated
-    const uint4 first = __ldg(reinterpret_cast<const uint4 *>(src + rot.first));
-    const uint4 second = __ldg(reinterpret_cast<const uint4 *>(src + rot.second));
-    float x[8], y[8];
-    unpack_half8(first, x);
-    unpack_half8(second, y);
-    if (rot.rotated && !is_v) rotate_item(x, y, c, s, INTERLEAVED);
-    if (is_q) {
-      __half *dst = qo + static_cast<size_t>(head) * D;
-      store_piece<KV_F16>(dst, rot.first, x, 1.f);
-      store_piece<KV_F16>(dst, rot.second, y, 1.f);
-    } else {
-      uint8_t *dst = (is_v ? vc : kc) + static_cast<size_t>(kv_head) * D * ELT;
-      float scale = a.scale;
-      if constexpr (KV != KV_F16 && SCALES != SCALE_SCALAR) {
-        const size_t si = (SCALES == SCALE_PER_HEAD)
-                              ? kv_head
-                              : static_cast<size_t>(slot / a.block_size) * a.num_kv_heads + kv_head;
-        scale = __ldg((is_v ? a.v_scales : a.k_scales) + si);
+  for (uint32_t first = head0; first < total; first += kRopeBatch * heads_per_pass) {
+    if (first != head0) load(first);
+#pragma unroll
+    for (uint32_t i = 0; i < kRopeBatch; ++i) {
+      const uint32_t head = first + i * heads_per_pass;
+      if (head >= total) break;
+      const bool is_v = head >= rotated_heads;
+      const bool is_q = head < a.num_heads;
+      const uint32_t kv_head = is_v ? head - rotated_heads : head - a.num_heads; // of K and V rows
+      float x[8], y[8];
+      unpack_half8(raw[i][0], x);
+      unpack_half8(raw[i][1], y);
+      if (rot.rotated && !is_v) rotate_item(x, y, c, s, INTERLEAVED); // V rows take the same two pieces
+      if (is_q) {
+        __half *dst = qo + static_cast<size_t>(head) * D;
+        *reinterpret_cast<uint4 *>(dst + rot.first) = pack_half8(x);
+        *reinterpret_cast<uint4 *>(dst + rot.second) = pack_half8(y);
+      } else {
+        uint8_t *dst = (is_v ? vc : kc) + static_cast<size_t>(kv_head) * D * ELT;
+        float scale = a.scale;
+        if constexpr (KV != KV_F16 && SCALES != SCALE_SCALAR) {
+          const size_t si = (SCALES == SCALE_PER_HEAD)
+                                ? kv_head
+                                : static_cast<size_t>(slot / a.block_size) * a.num_kv_heads + kv_head;
+          scale = __ldg((is_v ? a.v_scales : a.k_scales) + si);
+        }
+        const Divider by(scale);
+        store_piece<KV>(dst, rot.first, x, by);
+        store_piece<KV>(dst, rot.second, y, by);
       }
-      store_piece<KV>(dst, rot.first, x, scale);
-      store_piece<KV>(dst, rot.second, y, scale);
     }
   }
 }

@@ -23,11 +23,16 @@ from . import _shim
 ENTRY = "launch_kernels_diff"
 
 
+def _kv_dtype(cache: torch.Tensor) -> int:
+    return _shim._kv_dtype_of(cache, cache.dtype != torch.float16, cache.dtype == torch.int8)
+
+
 def scratch(query: torch.Tensor, key_cache: torch.Tensor, max_context_len: int):
     """(max_logits, exp_sums, tem_output) for calls of this shape: float32 [S, 2 H, NP], the same, and
     [S, 2 H, NP, 2 D].  NP sets how finely a context is split; any NP >= 1 gives a correct result."""
     s, h2, d = query.shape
-    npart = int(_cabi.load_library().pa_diff_num_partitions(s, key_cache.size(2), d, max(0, int(max_context_len))))
+    kv_dtype = _kv_dtype(key_cache)
+    npart = int(_cabi.load_library().pa_diff_num_partitions(s, key_cache.size(2), d, max(0, int(max_context_len)), kv_dtype))
     _shim._require(npart > 0, "Unsupported head size or number of KV heads")
     stats = torch.empty(2, s, h2, npart, dtype=torch.float32, device=query.device)
     return stats[0], stats[1], torch.empty(s, h2, npart, 2 * d, dtype=torch.float32, device=query.device)
@@ -79,7 +84,7 @@ def params(max_logits, exp_sums, tem_output, output, query, key_cache, value_cac
     p.max_context_len = max(0, min(int(max_context_len), 0xFFFFFFFF))
     p.num_blocks, p.sm_scale, p.fp8_scale = key_cache.size(0), float(sm_scale), float(kv_scale)
     fp16 = key_cache.dtype == torch.float16
-    p.kv_dtype = _shim._kv_dtype_of(key_cache, not fp16, key_cache.dtype == torch.int8)
+    p.kv_dtype = _kv_dtype(key_cache)
     per_head, per_block = (key_cache.size(2),), (key_cache.size(0), key_cache.size(2))
     for name, t, shape in (("k_scale_per_head", k_scale_per_head, per_head), ("v_scale_per_head", v_scale_per_head, per_head),
                            ("k_scale_per_block", k_scale_per_block, per_block),

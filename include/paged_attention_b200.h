@@ -198,9 +198,9 @@ PA_API int launch_kernels_int8_reduce(const pa_params *p, void *stream, float *u
  *   tmp_out        fp32 [num_seqs, 2 H, max_num_partitions, 2 * head_size]
  *   kv_dtype       any pa_kv_dtype; scales as in the FP8 and int8 entry points, per cache head
  *   sinks, alibi_slopes, softcap  must be off
- * A context is cut into at most max_num_partitions partitions of P tokens, P the smallest power of two
- * from 64 on with P * max_num_partitions >= max_context_len; the last one is open-ended, so the result
- * never depends on max_context_len. */
+ * A context is cut into at most max_num_partitions partitions of P tokens, P = max_context_len /
+ * max_num_partitions rounded up to a multiple of 64; the last one is open-ended, so a result never
+ * misses a token whatever max_context_len says. */
 typedef struct pa_diff_params {
   pa_params attn;
   const float *lambdas;     /* fp32 [H]: the learned weight of the second map */
@@ -217,10 +217,11 @@ typedef struct pa_diff_params {
 PA_API int launch_kernels_diff(const pa_diff_params *p, void *stream, float *us_out);
 
 /* Partitions that launch_kernels_diff is fastest with (the max_num_partitions to size its scratch
- * for): 512-token partitions, shorter ones while the batch does not fill the GPU.  num_kv_heads is
- * that of the cache (2 HK); 0 if the head size or an odd number of KV heads is not supported. */
+ * for): partitions of half a megabyte for a large batch, otherwise as many as fill whole rounds of the
+ * GPU.  num_kv_heads is that of the cache (2 HK), kv_dtype a pa_kv_dtype; 0 if the head size, the type or
+ * an odd number of KV heads is not supported. */
 PA_API uint32_t pa_diff_num_partitions(uint32_t num_seqs, uint32_t num_kv_heads, uint32_t head_size,
-                                       uint32_t max_context_len);
+                                       uint32_t max_context_len, int32_t kv_dtype);
 
 /* Size in bytes of the scratch array built into the library for
  * launch_kernels_reduce_static_scratch (32 MiB, held by every GPU that loads the library). */

@@ -155,6 +155,19 @@ PA_DEV void fp8x4_to_half2x2(uint32_t v, uint32_t &lo01, uint32_t &hi23) {
   }
 }
 
+// K fragments: as fp8x4_to_half2x2, but an integer code c becomes the half (c + 128) * 2^-24, a
+// subnormal whose bits are the biased byte itself.
+template <int KV>
+PA_DEV void key_codes_to_half2x2(uint32_t v, uint32_t &lo01, uint32_t &hi23) {
+  if constexpr (KV == 3) {
+    const uint32_t u = v ^ 0x80808080u;
+    lo01 = __byte_perm(u, 0u, 0x4140);
+    hi23 = __byte_perm(u, 0u, 0x4342);
+  } else {
+    fp8x4_to_half2x2<KV>(v, lo01, hi23);
+  }
+}
+
 // bytes (0,2) -> even, bytes (1,3) -> odd   (V fragments after a 16-bit transposing load)
 template <int KV>
 PA_DEV void fp8x4_to_even_odd_half2(uint32_t v, uint32_t &even, uint32_t &odd) {
@@ -187,6 +200,14 @@ PA_DEV void mbar_arrive_expect_tx(uint64_t *bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)),
                "r"(bytes)
                : "memory");
+}
+// Asynchronous 4-byte copy global -> shared memory, and an arrival on `bar` once all copies that
+// this thread has issued so are done (the arrival is counted in the barrier's initial count).
+PA_DEV void copy_async_4(void *dst_smem, const void *src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst_smem)), "l"(src) : "memory");
+}
+PA_DEV void mbar_arrive_after_copies(uint64_t *bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 PA_DEV bool mbar_try_wait(uint64_t *bar, uint32_t parity) {
   uint32_t ok;

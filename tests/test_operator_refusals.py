@@ -180,10 +180,13 @@ def test_differential_attention(lib):
 
 def test_diff_partition_counts(lib):
     n = lib.pa_diff_num_partitions
-    assert n(1, 3, 128, 1000) == 0 and n(1, 2, 96, 1000) == 0 and n(1, 0, 128, 1000) == 0
-    assert n(4, 8, 128, 0) == 1 and n(4, 8, 128, 1) == 1
-    assert n(1000, 8, 128, 1024) == 2       # a batch that fills the GPU: 512-token partitions
-    assert n(1, 2, 64, 1000) == 16          # a lone short sequence: the shortest ones
-    assert n(1, 8, 128, 2 ** 31) == 65535
-    sizes = [n(2, 8, 128, c) for c in range(1, 5000, 97)]
-    assert all(64 * s >= c for s, c in zip(sizes, range(1, 5000, 97)) if s < 65535)
+    f16, e4m3 = _cabi.KV_F16, _cabi.KV_FP8_E4M3
+    assert n(1, 3, 128, 1000, f16) == 0 and n(1, 2, 96, 1000, f16) == 0 and n(1, 0, 128, 1000, f16) == 0 and n(1, 2, 64, 9, 7) == 0
+    assert n(4, 8, 128, 0, f16) == 1 and n(4, 8, 128, 1, f16) == 1
+    assert n(3000, 8, 128, 1024, e4m3) == 2 and n(3000, 8, 128, 1024, f16) == 4  # a large batch: items of 512 KB
+    assert n(1, 2, 64, 1000, e4m3) == 16          # a lone short sequence: 64 tokens
+    assert n(2, 8, 128, 65536, e4m3) == 74        # 4 units: 296 items, one for every resident CTA
+    assert n(1000, 4, 128, 2 ** 27, f16) == 65535
+    for seqs in (1, 3, 40, 500):
+        for ctx in (1, 63, 700, 9000, 200000):
+            assert 1 <= n(seqs, 8, 64, ctx, e4m3) <= -(-ctx // 64)
