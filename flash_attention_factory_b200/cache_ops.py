@@ -15,7 +15,9 @@ import ctypes
 
 import torch
 
-from . import _cabi
+from . import _cabi, _launch
+
+_F16 = torch.float16
 
 
 def _kv_dtype(cache: torch.Tensor) -> int:
@@ -84,56 +86,56 @@ def reshape_and_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.T
         _cabi.check(lib.pa_reshape_and_cache(ctypes.byref(p), ctypes.c_void_p(stream)))
 
 
-def _require(cond: bool, msg: str) -> None:
-    if not cond:
-        raise RuntimeError(msg)
-
-
-def _token_rows(t: torch.Tensor, name: str, device) -> int:
+def _token_rows(t: torch.Tensor, name: str, index: int) -> int:
     """Checks fp16 rows [T, heads, D] whose tokens may lie any stride apart (slices of one projection's
     output); returns that stride in elements."""
-    _require(t.is_cuda and t.device == device and t.dtype == torch.float16 and t.dim() == 3,
-             f"{name} must be a float16 tensor [tokens, heads, head_size] on the cache's device")
-    _require(t.stride(2) == 1 and (t.size(1) == 1 or t.stride(1) == t.size(2)),
-             f"the heads of a token of {name} must be contiguous")
-    stride = t.stride(0) if t.size(0) > 1 else t.size(1) * t.size(2)
-    _require(stride >= 0 and stride % 8 == 0, f"the token stride of {name} must be a multiple of 8 elements")
+    if t.dtype is not _F16 or t.dim() != 3 or t.get_device() != index:
+        raise RuntimeError(f"{name} must be a float16 tensor [tokens, heads, head_size] on the cache's device")
+    tokens, heads, d = t.shape
+    stride, head_stride, last = t.stride()
+    if last != 1 or (heads != 1 and head_stride != d):
+        raise RuntimeError(f"the heads of a token of {name} must be contiguous")
+    if tokens <= 1:
+        return heads * d
+    if stride < 0 or stride % 8 != 0:
+        raise RuntimeError(f"the token stride of {name} must be a multiple of 8 elements")
     return stride
 
 
-def _check_caches(key, value, key_cache, value_cache) -> None:
-    _require(key_cache.is_cuda and key_cache.is_contiguous() and value_cache.is_contiguous()
-             and value_cache.device == key_cache.device, "the caches must be contiguous CUDA tensors on one device "
-             "(no CPU fallback exists)")
-    _require(key_cache.dim() == 4 and key_cache.shape == value_cache.shape and key_cache.dtype == value_cache.dtype,
-             "key_cache and value_cache must match")
-    _require(key.shape == value.shape and tuple(key_cache.shape[2:]) == tuple(key.shape[1:]),
-             "cache must be [num_blocks, block_size, num_kv_heads, head_size]")
+def _check_caches(key, value, key_cache, value_cache) -> int:
+    """Checks the caches against the rows; returns the device index."""
+    index = key_cache.get_device()
+    if index < 0 or value_cache.get_device() != index or not (key_cache.is_contiguous() and value_cache.is_contiguous()):
+        raise RuntimeError("the caches must be contiguous CUDA tensors on one device (no CPU fallback exists)")
+    shape = key_cache.shape
+    if len(shape) != 4 or shape != value_cache.shape or key_cache.dtype is not value_cache.dtype:
+        raise RuntimeError("key_cache and value_cache must match")
+    rows = key.shape
+    if rows != value.shape or shape[2:] != rows[1:]:
+        raise RuntimeError("cache must be [num_blocks, block_size, num_kv_heads, head_size]")
+    return index
 
 
-def _check_rotation(cos_sin, device) -> None:
-    _require(cos_sin.dtype == torch.float32 and cos_sin.dim() == 2 and cos_sin.is_contiguous() and cos_sin.device == device,
-             "cos_sin must be a contiguous float32 tensor [max_position, rotary_dim] on the cache's device")
+def _check_rotation(cos_sin, index: int) -> None:
+    if (cos_sin.dtype is not torch.float32 or cos_sin.dim() != 2 or not cos_sin.is_contiguous()
+            or cos_sin.get_device() != index):
+        raise RuntimeError("cos_sin must be a contiguous float32 tensor [max_position, rotary_dim] on the cache's device")
 
 
-def _check_queries(p, query, query_out, key) -> None:
+def _check_queries(p, query, query_out, key, index: int) -> None:
     """Fills the query part of an argument block."""
-    _require((query is None) == (query_out is None), "query and query_out must be given together")
-    if query is None:
+    if query is None and query_out is None:
         return
-    p.query_token_stride = _token_rows(query, "query", key.device)
-    _require(query.size(0) == key.size(0) and query.size(2) == key.size(2), "query and key must have the same tokens and head_size")
-    _require(query_out.shape == query.shape and query_out.dtype == torch.float16 and query_out.is_contiguous()
-             and query_out.device == key.device, "query_out must be a contiguous float16 tensor of query's shape")
-    p.num_heads, p.query, p.query_out = query.size(1), query.data_ptr(), query_out.data_ptr()
-
-
-def _call(fn, p, device) -> None:
-    """Runs a writer on torch's current stream of `device`, with that device current."""
-    if torch.cuda.current_device() != device.index:
-        with torch.cuda.device(device):
-            return _call(fn, p, torch.device("cuda", torch.cuda.current_device()))
-    _cabi.check(fn(ctypes.byref(p), ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)))
+    if query is None or query_out is None:
+        raise RuntimeError("query and query_out must be given together")
+    p.query_token_stride = _token_rows(query, "query", index)
+    shape, rows = query.shape, key.shape
+    if shape[0] != rows[0] or shape[2] != rows[2]:
+        raise RuntimeError("query and key must have the same tokens and head_size")
+    if (query_out.shape != shape or query_out.dtype is not _F16 or not query_out.is_contiguous()
+            or query_out.get_device() != index):
+        raise RuntimeError("query_out must be a contiguous float16 tensor of query's shape")
+    p.num_heads, p.query, p.query_out = shape[1], query.data_ptr(), query_out.data_ptr()
 
 
 def rope_and_cache(query, key: torch.Tensor, value: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor,
@@ -153,28 +155,30 @@ def rope_and_cache(query, key: torch.Tensor, value: torch.Tensor, positions: tor
     or whose slot or position is out of range, is skipped: its cache and query_out rows stay as they
     were.  Asynchronous on torch's current stream.
     """
-    _check_caches(key, value, key_cache, value_cache)
-    device = key_cache.device
+    index = _check_caches(key, value, key_cache, value_cache)
     p = _cabi.PaRopeCacheParams()
-    p.key_token_stride = _token_rows(key, "key", device)
-    p.value_token_stride = _token_rows(value, "value", device)
-    t = key.size(0)
-    for name, x in (("slot_mapping", slot_mapping), ("positions", positions)):
-        _require(x.dtype == torch.int64 and x.numel() == t and x.is_contiguous() and x.device == device,
-                 f"{name} must be int64 with one entry per token on the cache's device")
-    _check_rotation(cos_sin, device)
-    _check_queries(p, query, query_out, key)
+    p.key_token_stride = _token_rows(key, "key", index)
+    p.value_token_stride = _token_rows(value, "value", index)
+    num_blocks, block_size, kv_heads, head_size = key_cache.shape
+    tokens = key.shape[0]
+    for x in (slot_mapping, positions):
+        if x.dtype is not torch.int64 or x.numel() != tokens or not x.is_contiguous() or x.get_device() != index:
+            raise RuntimeError("slot_mapping and positions must be int64 with one entry per token on the cache's device")
+    _check_rotation(cos_sin, index)
+    _check_queries(p, query, query_out, key, index)
     c = p.cache
     c.key, c.value = key.data_ptr(), value.data_ptr()
     c.key_cache, c.value_cache = key_cache.data_ptr(), value_cache.data_ptr()
     c.slot_mapping = slot_mapping.data_ptr()
-    c.num_tokens, c.num_kv_heads, c.head_size = t, key.size(1), key.size(2)
-    c.block_size, c.num_blocks = key_cache.size(1), key_cache.size(0)
+    c.num_tokens, c.num_kv_heads, c.head_size = tokens, kv_heads, head_size
+    c.block_size, c.num_blocks = block_size, num_blocks
     c.fp8_scale, c.kv_dtype = float(fp8_scale), _kv_dtype(key_cache)
-    _set_scales(c, key, key_cache, k_scale_per_head, v_scale_per_head, k_scale_per_block, v_scale_per_block)
+    if not (k_scale_per_head is v_scale_per_head is k_scale_per_block is v_scale_per_block is None):
+        _set_scales(c, key, key_cache, k_scale_per_head, v_scale_per_head, k_scale_per_block, v_scale_per_block)
     p.positions, p.cos_sin = positions.data_ptr(), cos_sin.data_ptr()
-    p.max_position, p.rotary_dim, p.interleaved = cos_sin.size(0), cos_sin.size(1), int(interleaved)
-    _call(_cabi.load_library().pa_rope_and_cache, p, device)
+    p.max_position, p.rotary_dim = cos_sin.shape
+    p.interleaved = int(interleaved)
+    _launch.call(_cabi.load_library().pa_rope_and_cache, p, index)
 
 
 def append_block_scaled(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
@@ -196,33 +200,38 @@ def append_block_scaled(key: torch.Tensor, value: torch.Tensor, key_cache: torch
     behind the last sequence, and tokens whose position lies outside the table row or the rotation table, are
     skipped.  Asynchronous on torch's current stream.
     """
-    _check_caches(key, value, key_cache, value_cache)
-    device = key_cache.device
+    index = _check_caches(key, value, key_cache, value_cache)
     p = _cabi.PaBlockScaledParams()
-    p.key_token_stride = _token_rows(key, "key", device)
-    p.value_token_stride = _token_rows(value, "value", device)
-    nb, bs, hk, d = key_cache.shape
-    for name, t in (("k_scale_per_block", k_scale_per_block), ("v_scale_per_block", v_scale_per_block)):
-        _require(t.dtype == torch.float32 and tuple(t.shape) == (nb, hk) and t.is_contiguous() and t.device == device,
-                 f"{name} must be a contiguous float32 tensor [num_blocks, num_kv_heads] on the cache's device")
-    _require(block_tables.dim() == 2 and block_tables.size(0) == context_lens.numel(),
-             "block_tables must be [num_seqs, max_blocks_per_seq] with one context length per row")
-    for name, t in (("block_tables", block_tables), ("context_lens", context_lens), ("cu_tokens", cu_tokens)):
-        _require(t is None or (t.dtype == torch.int32 and t.is_contiguous() and t.device == device),
-                 f"{name} must be contiguous int32 on the cache's device")
+    p.key_token_stride = _token_rows(key, "key", index)
+    p.value_token_stride = _token_rows(value, "value", index)
+    num_blocks, block_size, kv_heads, head_size = key_cache.shape
+    for t in (k_scale_per_block, v_scale_per_block):
+        if (t.dtype is not torch.float32 or t.shape != (num_blocks, kv_heads) or not t.is_contiguous()
+                or t.get_device() != index):
+            raise RuntimeError("k_scale_per_block and v_scale_per_block must be contiguous float32 tensors "
+                               "[num_blocks, num_kv_heads] on the cache's device")
     seqs = context_lens.numel()
-    _require(cu_tokens is None or cu_tokens.numel() == seqs + 1, "cu_tokens must have num_seqs + 1 entries")
-    _require(query is None or cos_sin is not None, "queries are only taken to be rotated: cos_sin is missing")
+    if block_tables.dim() != 2 or block_tables.shape[0] != seqs:
+        raise RuntimeError("block_tables must be [num_seqs, max_blocks_per_seq] with one context length per row")
+    for t in (block_tables, context_lens, cu_tokens):
+        if t is not None and (t.dtype is not torch.int32 or not t.is_contiguous() or t.get_device() != index):
+            raise RuntimeError("block_tables, context_lens and cu_tokens must be contiguous int32 on the cache's device")
+    if cu_tokens is not None:
+        if cu_tokens.numel() != seqs + 1:
+            raise RuntimeError("cu_tokens must have num_seqs + 1 entries")
+        p.cu_tokens = cu_tokens.data_ptr()
     if cos_sin is not None:
-        _check_rotation(cos_sin, device)
-        p.cos_sin, p.max_position, p.rotary_dim = cos_sin.data_ptr(), cos_sin.size(0), cos_sin.size(1)
-    _check_queries(p, query, query_out, key)
+        _check_rotation(cos_sin, index)
+        p.cos_sin = cos_sin.data_ptr()
+        p.max_position, p.rotary_dim = cos_sin.shape
+    elif query is not None:
+        raise RuntimeError("queries are only taken to be rotated: cos_sin is missing")
+    _check_queries(p, query, query_out, key, index)
     p.key, p.value = key.data_ptr(), value.data_ptr()
     p.key_cache, p.value_cache = key_cache.data_ptr(), value_cache.data_ptr()
     p.k_scale_per_block, p.v_scale_per_block = k_scale_per_block.data_ptr(), v_scale_per_block.data_ptr()
     p.block_tables, p.context_lens = block_tables.data_ptr(), context_lens.data_ptr()
-    p.cu_tokens = cu_tokens.data_ptr() if cu_tokens is not None else None
-    p.num_seqs, p.num_tokens, p.num_kv_heads, p.head_size = seqs, key.size(0), hk, d
-    p.block_size, p.max_blocks_per_seq, p.num_blocks = bs, block_tables.size(1), nb
+    p.num_seqs, p.num_tokens, p.num_kv_heads, p.head_size = seqs, key.shape[0], kv_heads, head_size
+    p.block_size, p.max_blocks_per_seq, p.num_blocks = block_size, block_tables.shape[1], num_blocks
     p.kv_dtype, p.interleaved = _kv_dtype(key_cache), int(interleaved)
-    _call(_cabi.load_library().pa_append_block_scaled, p, device)
+    _launch.call(_cabi.load_library().pa_append_block_scaled, p, index)

@@ -10,7 +10,9 @@ from __future__ import annotations
 
 import torch
 
-from .. import _cabi
+from .. import _cabi, _launch
+
+_F16, _F32, _I32 = torch.float16, torch.float32, torch.int32
 
 
 def _require(cond: bool, msg: str) -> None:
@@ -46,33 +48,43 @@ def build_params(max_logits, exp_sums, tem_output, output, debug_output, query, 
     reference (paged_attention_kernel_loop.hpp:175-178,329-342).  ``int8`` (with ``fp8``, whose
     scale arguments it shares) selects the integer cache.
     """
-    _require(query.is_cuda, "paged attention needs CUDA tensors (no CPU fallback exists)")
+    if not query.is_cuda:
+        raise RuntimeError("paged attention needs CUDA tensors (no CPU fallback exists)")
     # the reference's data_ptr<float>() calls reject other dtypes (paged_attention_loop.cpp:47-52)
-    for name, t in (("max_logits", max_logits), ("exp_sums", exp_sums), ("alibi_slopes", alibi_slopes),
-                    ("debug_output", debug_output)):
-        if name == "debug_output" and t is None:
-            continue  # callers of this package that have no debug tensor pass None
-        _require(t.dtype == torch.float32, f"expected scalar type Float but found {t.dtype} ({name})")
-    _require(query.dtype == torch.float16 and output.dtype == torch.float16,
-             "query and output must be float16")
-    _require(block_tables.dtype == torch.int32 and context_lens.dtype == torch.int32,
-             "block_tables and context_lens must be int32")
-    _require(query.dim() == 3 and key_cache.dim() == 4 and block_tables.dim() == 2
-             and max_logits.dim() == 3, "unexpected tensor rank")
-    _require(key_cache.shape == value_cache.shape and key_cache.dtype == value_cache.dtype,
-             "key_cache and value_cache must have the same shape and dtype")
-    tensors = [max_logits, exp_sums, tem_output, output, query, key_cache, value_cache,
-               block_tables, context_lens]
-    if sinks is not None:
-        _require(sinks.dtype == torch.float16, "sinks must be float16")
-        tensors.append(sinks)
-    for t in tensors:
-        _require(t.is_contiguous(), "all tensors must be contiguous")
-        _require(t.device == query.device, "all tensors must be on the same device")
-    _require(key_cache.size(1) == block_size, "block_size does not match key_cache.size(1)")
-    _require(key_cache.size(3) == query.size(2), "head_size of cache and query differ")
-    _require(context_lens.numel() == query.size(0) and block_tables.size(0) == query.size(0),
-             "context_lens / block_tables do not match the number of sequences")
+    if (max_logits.dtype is not _F32 or exp_sums.dtype is not _F32 or alibi_slopes.dtype is not _F32
+            or (debug_output is not None and debug_output.dtype is not _F32)):
+        # callers of this package that have no debug tensor pass None
+        for name, t in (("max_logits", max_logits), ("exp_sums", exp_sums), ("alibi_slopes", alibi_slopes),
+                        ("debug_output", debug_output)):
+            if t is not None:
+                _require(t.dtype == torch.float32, f"expected scalar type Float but found {t.dtype} ({name})")
+    if query.dtype is not _F16 or output.dtype is not _F16:
+        raise RuntimeError("query and output must be float16")
+    if block_tables.dtype is not _I32 or context_lens.dtype is not _I32:
+        raise RuntimeError("block_tables and context_lens must be int32")
+    if query.dim() != 3 or key_cache.dim() != 4 or block_tables.dim() != 2 or max_logits.dim() != 3:
+        raise RuntimeError("unexpected tensor rank")
+    num_blocks, rows, kv_heads, cache_head_size = cache_shape = key_cache.shape
+    if cache_shape != value_cache.shape or key_cache.dtype is not value_cache.dtype:
+        raise RuntimeError("key_cache and value_cache must have the same shape and dtype")
+    if sinks is not None and sinks.dtype is not _F16:
+        raise RuntimeError("sinks must be float16")
+    index = query.get_device()
+    for t in (max_logits, exp_sums, tem_output, output, query, key_cache, value_cache, block_tables, context_lens, sinks):
+        if t is None:
+            continue
+        if not t.is_contiguous():
+            raise RuntimeError("all tensors must be contiguous")
+        if t.get_device() != index:
+            raise RuntimeError("all tensors must be on the same device")
+    num_seqs, num_heads, head_size = query.shape
+    table_rows, table_columns = block_tables.shape
+    if rows != block_size:
+        raise RuntimeError("block_size does not match key_cache.size(1)")
+    if cache_head_size != head_size:
+        raise RuntimeError("head_size of cache and query differ")
+    if context_lens.numel() != num_seqs or table_rows != num_seqs:
+        raise RuntimeError("context_lens / block_tables do not match the number of sequences")
 
     p = _cabi.PaParams()
     p.out = output.data_ptr()
@@ -85,32 +97,35 @@ def build_params(max_logits, exp_sums, tem_output, output, debug_output, query, 
     p.sinks = sinks.data_ptr() if sinks is not None else None
     p.block_tables = block_tables.data_ptr()
     p.context_lens = context_lens.data_ptr()
-    p.num_seqs = query.size(0)
-    p.num_heads = query.size(1)
-    p.head_size = query.size(2)
-    p.num_kv_heads = key_cache.size(2)
-    p.max_num_partitions = max_logits.size(2)
-    p.max_blocks_per_seq = block_tables.size(1)
+    p.num_seqs = num_seqs
+    p.num_heads = num_heads
+    p.head_size = head_size
+    p.num_kv_heads = kv_heads
+    p.max_num_partitions = max_logits.shape[2]
+    p.max_blocks_per_seq = table_columns
     p.block_size = int(block_size)
     p.num_queries_per_tokens = int(num_queries_per_tokens)
     p.max_context_len = max(0, min(int(max_context_len), 0xFFFFFFFF))
-    p.num_blocks = key_cache.size(0)
+    p.num_blocks = num_blocks
     p.sm_scale = float(sm_scale)
     p.fp8_scale = float(fp8_scale)
     p.kv_dtype = _kv_dtype_of(key_cache, fp8, int8)
-    for name, t in (("k_scale_per_head", k_scale_per_head), ("v_scale_per_head", v_scale_per_head)):
-        if t is not None:
-            _require(fp8, "per-head scales belong to the FP8 and int8 operators")
-            _require(t.dtype == torch.float32 and t.is_contiguous() and t.device == query.device
-                     and t.numel() == key_cache.size(2), f"{name} must be float32 [num_kv_heads] on the device")
-            setattr(p, name, t.data_ptr())
-    for name, t in (("k_scale_per_block", k_scale_per_block), ("v_scale_per_block", v_scale_per_block)):
-        if t is not None:
-            _require(fp8, "per-block scales belong to the FP8 and int8 operators")
-            _require(t.dtype == torch.float32 and t.is_contiguous() and t.device == query.device
-                     and tuple(t.shape) == (key_cache.size(0), key_cache.size(2)),
-                     f"{name} must be float32 [num_blocks, num_kv_heads] on the device")
-            setattr(p, name, t.data_ptr())
+    if k_scale_per_head is not None or v_scale_per_head is not None:
+        for name, t in (("k_scale_per_head", k_scale_per_head), ("v_scale_per_head", v_scale_per_head)):
+            if t is not None:
+                _require(fp8, "per-head scales belong to the FP8 and int8 operators")
+                _require(t.dtype == torch.float32 and t.is_contiguous() and t.device == query.device
+                         and t.numel() == kv_heads, f"{name} must be float32 [num_kv_heads] on the device")
+                setattr(p, name, t.data_ptr())
+    if k_scale_per_block is not None or v_scale_per_block is not None:
+        for name, t in (("k_scale_per_block", k_scale_per_block), ("v_scale_per_block", v_scale_per_block)):
+            if t is not None:
+                if not fp8:
+                    raise RuntimeError("per-block scales belong to the FP8 and int8 operators")
+                if (t.dtype is not _F32 or not t.is_contiguous() or t.get_device() != index
+                        or t.shape != (num_blocks, kv_heads)):
+                    raise RuntimeError(f"{name} must be float32 [num_blocks, num_kv_heads] on the device")
+                setattr(p, name, t.data_ptr())
     # opt-in only: by default alibi_slopes and softcap are ignored, as in the reference
     if use_alibi:
         _require(alibi_slopes.is_cuda and alibi_slopes.is_contiguous()
@@ -139,6 +154,5 @@ def run_entry(entry: str, p: _cabi.PaParams, device: torch.device) -> list[float
 
 def enqueue_entry(entry: str, p: _cabi.PaParams, device: torch.device) -> None:
     """Asynchronous launch on torch's current stream (no timing, no host sync)."""
-    with torch.cuda.device(device):
-        stream = torch.cuda.current_stream(device).cuda_stream
-        _cabi.launch(entry, p, stream, timed=False)
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    _launch.call(getattr(_cabi.load_library(), entry), p, index, None)

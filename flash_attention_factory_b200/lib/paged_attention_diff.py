@@ -17,8 +17,10 @@ import ctypes
 
 import torch
 
-from .. import _cabi
+from .. import _cabi, _launch
 from . import _shim
+
+_F32 = torch.float32
 
 ENTRY = "launch_kernels_diff"
 
@@ -43,72 +45,74 @@ def params(max_logits, exp_sums, tem_output, output, query, key_cache, value_cac
            norm_scale=1.0, k_scale_per_head=None, v_scale_per_head=None, k_scale_per_block=None,
            v_scale_per_block=None) -> _cabi.PaDiffParams:
     """The checked argument block (`pa_diff_params`) of an ``enqueue`` call with these arguments."""
-    require = _shim._require
-    require(query.is_cuda, "paged attention needs CUDA tensors (no CPU fallback exists)")
-    require(query.dim() == 3 and key_cache.dim() == 4 and block_tables.dim() == 2 and max_logits.dim() == 3,
-            "unexpected tensor rank")
+    index = query.get_device()
+    if index < 0:
+        raise RuntimeError("paged attention needs CUDA tensors (no CPU fallback exists)")
+    if query.dim() != 3 or key_cache.dim() != 4 or block_tables.dim() != 2 or max_logits.dim() != 3:
+        raise RuntimeError("unexpected tensor rank")
     s, h2, d = query.shape
-    npart, device = max_logits.size(2), query.device
-    require(h2 % 2 == 0 and key_cache.size(2) % 2 == 0 and key_cache.size(2) > 0,
-            "differential attention needs query heads and KV heads in pairs")
-    require(h2 % key_cache.size(2) == 0, "the number of query heads must be a multiple of the number of KV heads")
-    require(query.dtype == torch.float16 and output.dtype == torch.float16, "query and output must be float16")
-    require(tuple(output.shape) == (s, h2 // 2, 2 * d), "output must be [num_seqs, H, 2 * head_size]")
-    require(max_logits.dtype == exp_sums.dtype == tem_output.dtype == torch.float32, "the scratch must be float32")
-    require(tuple(max_logits.shape) == (s, h2, npart) and tuple(exp_sums.shape) == (s, h2, npart)
-            and tem_output.numel() >= s * h2 * npart * 2 * d,
-            "the scratch must be [num_seqs, 2 H, NP] twice and [num_seqs, 2 H, NP, 2 * head_size]")
-    require(block_tables.dtype == torch.int32 and context_lens.dtype == torch.int32,
-            "block_tables and context_lens must be int32")
-    require(context_lens.numel() == s and block_tables.size(0) == s,
-            "context_lens / block_tables do not match the number of sequences")
-    require(key_cache.shape == value_cache.shape and key_cache.dtype == value_cache.dtype,
-            "key_cache and value_cache must have the same shape and dtype")
-    require(key_cache.size(1) == block_size, "block_size does not match key_cache.size(1)")
-    require(key_cache.size(3) == d, "head_size of cache and query differ")
-    require(lambdas.dtype == torch.float32 and lambdas.numel() == h2 // 2, "lambdas must be float32 [H]")
-    require(norm_weight is None or (norm_weight.dtype == torch.float32 and norm_weight.numel() == 2 * d),
-            "norm_weight must be float32 [2 * head_size]")
+    num_blocks, rows, kv_heads, cache_head_size = cache_shape = key_cache.shape
+    table_rows, table_columns = block_tables.shape
+    npart = max_logits.shape[2]
+    if h2 % 2 or kv_heads % 2 or kv_heads == 0:
+        raise RuntimeError("differential attention needs query heads and KV heads in pairs")
+    if h2 % kv_heads:
+        raise RuntimeError("the number of query heads must be a multiple of the number of KV heads")
+    if query.dtype is not torch.float16 or output.dtype is not torch.float16:
+        raise RuntimeError("query and output must be float16")
+    if output.shape != (s, h2 // 2, 2 * d):
+        raise RuntimeError("output must be [num_seqs, H, 2 * head_size]")
+    if max_logits.dtype is not _F32 or exp_sums.dtype is not _F32 or tem_output.dtype is not _F32:
+        raise RuntimeError("the scratch must be float32")
+    if (max_logits.shape != (s, h2, npart) or exp_sums.shape != (s, h2, npart)
+            or tem_output.numel() < s * h2 * npart * 2 * d):
+        raise RuntimeError("the scratch must be [num_seqs, 2 H, NP] twice and [num_seqs, 2 H, NP, 2 * head_size]")
+    if block_tables.dtype is not torch.int32 or context_lens.dtype is not torch.int32:
+        raise RuntimeError("block_tables and context_lens must be int32")
+    if context_lens.numel() != s or table_rows != s:
+        raise RuntimeError("context_lens / block_tables do not match the number of sequences")
+    if cache_shape != value_cache.shape or key_cache.dtype is not value_cache.dtype:
+        raise RuntimeError("key_cache and value_cache must have the same shape and dtype")
+    if rows != block_size:
+        raise RuntimeError("block_size does not match key_cache.size(1)")
+    if cache_head_size != d:
+        raise RuntimeError("head_size of cache and query differ")
+    if lambdas.dtype is not _F32 or lambdas.numel() != h2 // 2:
+        raise RuntimeError("lambdas must be float32 [H]")
+    if norm_weight is not None and (norm_weight.dtype is not _F32 or norm_weight.numel() != 2 * d):
+        raise RuntimeError("norm_weight must be float32 [2 * head_size]")
     for t in (max_logits, exp_sums, tem_output, output, query, key_cache, value_cache, block_tables, context_lens,
               lambdas, norm_weight):
-        require(t is None or (t.is_contiguous() and t.device == device), "all tensors must be contiguous and on the same device")
+        if t is not None and (not t.is_contiguous() or t.get_device() != index):
+            raise RuntimeError("all tensors must be contiguous and on the same device")
     q = _cabi.PaDiffParams()
     p = q.attn
     p.out, p.max_logits, p.exp_sums = output.data_ptr(), max_logits.data_ptr(), exp_sums.data_ptr()
     p.tmp_out, p.query = tem_output.data_ptr(), query.data_ptr()
     p.key_cache, p.value_cache = key_cache.data_ptr(), value_cache.data_ptr()
     p.block_tables, p.context_lens = block_tables.data_ptr(), context_lens.data_ptr()
-    p.num_seqs, p.num_heads, p.head_size, p.num_kv_heads = s, h2, d, key_cache.size(2)
-    p.max_num_partitions, p.max_blocks_per_seq = npart, block_tables.size(1)
-    p.block_size, p.num_queries_per_tokens = int(block_size), h2 // key_cache.size(2)
+    p.num_seqs, p.num_heads, p.head_size, p.num_kv_heads = s, h2, d, kv_heads
+    p.max_num_partitions, p.max_blocks_per_seq = npart, table_columns
+    p.block_size, p.num_queries_per_tokens = int(block_size), h2 // kv_heads
     p.max_context_len = max(0, min(int(max_context_len), 0xFFFFFFFF))
-    p.num_blocks, p.sm_scale, p.fp8_scale = key_cache.size(0), float(sm_scale), float(kv_scale)
-    fp16 = key_cache.dtype == torch.float16
+    p.num_blocks, p.sm_scale, p.fp8_scale = num_blocks, float(sm_scale), float(kv_scale)
     p.kv_dtype = _kv_dtype(key_cache)
-    per_head, per_block = (key_cache.size(2),), (key_cache.size(0), key_cache.size(2))
-    for name, t, shape in (("k_scale_per_head", k_scale_per_head, per_head), ("v_scale_per_head", v_scale_per_head, per_head),
-                           ("k_scale_per_block", k_scale_per_block, per_block),
-                           ("v_scale_per_block", v_scale_per_block, per_block)):
-        if t is not None:
-            require(not fp16, "scale arrays belong to FP8 and int8 caches")
-            require(t.dtype == torch.float32 and t.is_contiguous() and t.device == device and tuple(t.shape) == shape,
-                    f"{name} must be a contiguous float32 tensor of shape {shape} on the device")
-            setattr(p, name, t.data_ptr())
+    if not (k_scale_per_head is v_scale_per_head is k_scale_per_block is v_scale_per_block is None):
+        if key_cache.dtype == torch.float16:
+            raise RuntimeError("scale arrays belong to FP8 and int8 caches")
+        for name, t, shape in (("k_scale_per_head", k_scale_per_head, (kv_heads,)),
+                               ("v_scale_per_head", v_scale_per_head, (kv_heads,)),
+                               ("k_scale_per_block", k_scale_per_block, (num_blocks, kv_heads)),
+                               ("v_scale_per_block", v_scale_per_block, (num_blocks, kv_heads))):
+            if t is not None:
+                if t.dtype is not _F32 or not t.is_contiguous() or t.get_device() != index or t.shape != shape:
+                    raise RuntimeError(f"{name} must be a contiguous float32 tensor of shape {shape} on the device")
+                setattr(p, name, t.data_ptr())
     q.lambdas = lambdas.data_ptr()
     if norm_weight is not None:
         q.norm_weight, q.norm_eps = norm_weight.data_ptr(), float(norm_eps)
     q.norm_scale = float(norm_scale)
     return q
-
-
-def _launch(q: _cabi.PaDiffParams, device, timed: bool):
-    if torch.cuda.current_device() != device.index:
-        with torch.cuda.device(device):
-            return _launch(q, torch.device("cuda", torch.cuda.current_device()), timed)
-    us = (ctypes.c_float * 2)() if timed else None
-    stream = ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
-    _cabi.check(_cabi.load_library().launch_kernels_diff(ctypes.byref(q), stream, us))
-    return [float(us[0]), float(us[1])] if timed else None
 
 
 def enqueue(max_logits, exp_sums, tem_output, output, query, key_cache, value_cache, block_tables, context_lens,
@@ -123,9 +127,11 @@ def enqueue(max_logits, exp_sums, tem_output, output, query, key_cache, value_ca
                lambdas, sm_scale, kv_scale, block_size, max_context_len, norm_weight=norm_weight, norm_eps=norm_eps,
                norm_scale=norm_scale, k_scale_per_head=k_scale_per_head, v_scale_per_head=v_scale_per_head,
                k_scale_per_block=k_scale_per_block, v_scale_per_block=v_scale_per_block)
-    _launch(q, query.device, timed=False)
+    _launch.call(_cabi.load_library().launch_kernels_diff, q, query.get_device(), None)
 
 
 def run(*args, **kwargs) -> list[float]:
     """``enqueue``, blocking; returns device microseconds [attention, merge]."""
-    return _launch(params(*args, **kwargs), args[4].device, timed=True)
+    us = (ctypes.c_float * 2)()
+    _launch.call(_cabi.load_library().launch_kernels_diff, params(*args, **kwargs), args[4].get_device(), us)
+    return [float(us[0]), float(us[1])]
