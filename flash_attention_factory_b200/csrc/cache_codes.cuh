@@ -164,4 +164,72 @@ __device__ __forceinline__ void rotate_item(float (&x)[8], float (&y)[8], const 
   }
 }
 
+// ------------------------------------------------ the same on pairs of values (one instruction for two)
+__device__ __forceinline__ unsigned long long pair_bits(float2 v) {
+  return static_cast<unsigned long long>(__float_as_uint(v.x)) | (static_cast<unsigned long long>(__float_as_uint(v.y)) << 32);
+}
+__device__ __forceinline__ float2 bits_pair(unsigned long long v) {
+  return make_float2(__uint_as_float(static_cast<uint32_t>(v)), __uint_as_float(static_cast<uint32_t>(v >> 32)));
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)));
+  return bits_pair(r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pair_bits(a)), "l"(pair_bits(b)), "l"(pair_bits(c)));
+  return bits_pair(r);
+}
+
+struct Item2 {
+  float2 x[4], y[4]; // the item's two pieces of eight
+};
+
+__device__ __forceinline__ void unpack_item(const uint4 &first, const uint4 &second, Item2 &v) {
+  const __half2 *a = reinterpret_cast<const __half2 *>(&first);
+  const __half2 *b = reinterpret_cast<const __half2 *>(&second);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    v.x[j] = __half22float2(a[j]);
+    v.y[j] = __half22float2(b[j]);
+  }
+}
+
+// rotate_item with the table row's pieces read on the way; every product and sum is rounded as there
+__device__ __forceinline__ void rotate_item2(Item2 &v, const float *__restrict__ cosines, const float *__restrict__ sines,
+                                             bool interleaved) {
+  // u - v as fma(v, -1, u): a plain addition of two packed products is contracted into a fused multiply-add by
+  // the compiler, rounding modifiers or not
+  const float2 minus = make_float2(-1.f, -1.f), alternate = make_float2(-1.f, 1.f);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const float4 c4 = __ldg(reinterpret_cast<const float4 *>(cosines) + k);
+    const float4 s4 = __ldg(reinterpret_cast<const float4 *>(sines) + k);
+    if (!interleaved) {
+      const float2 c[2] = {make_float2(c4.x, c4.y), make_float2(c4.z, c4.w)};
+      const float2 s[2] = {make_float2(s4.x, s4.y), make_float2(s4.z, s4.w)};
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float2 a = v.x[2 * k + j], b = v.y[2 * k + j];
+        v.x[2 * k + j] = fma2(mul2(b, s[j]), minus, mul2(a, c[j]));
+        v.y[2 * k + j] = fma2(mul2(a, make_float2(-s[j].x, -s[j].y)), minus, mul2(b, c[j]));
+      }
+    } else {
+      const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+      float2 *p = (k == 0) ? v.x : v.y;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        p[j] = fma2(mul2(make_float2(p[j].y, p[j].x), make_float2(s[j], s[j])), alternate,
+                    mul2(p[j], make_float2(c[j], c[j])));
+    }
+  }
+}
+
+// Divider on a pair
+__device__ __forceinline__ float2 divide2(float2 x, float2 minus_s, float2 r) {
+  const float2 q = mul2(x, r);
+  return fma2(fma2(q, minus_s, x), r, q);
+}
+
 } // namespace pa
