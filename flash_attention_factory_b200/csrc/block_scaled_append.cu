@@ -202,15 +202,6 @@ __device__ __forceinline__ void requantise_rows(uint8_t *at, size_t step, uint32
   }
 }
 
-// The usual way: up to PASSES row groups of the warp are copied to its own corner of shared memory while the job before
-// is worked on, and are gone through there twice, for the maximum and for the codes.  (K is rotated both times: the
-// rotated rows as fp32 in registers cost the SM a third of its warps.)  Every lane reads back what it copied itself, so
-// nothing but its own copies has to be waited for.  The maximum of V is taken two fp16 values at a time.  The
-// maxima propagate NaNs, so an infinity or a NaN among the inputs shows in the result.  A lane without a row of its
-// own in a group takes the last row over again: it changes no maximum and is not stored.
-// Measured on 37 376 prompt tokens (8 KV heads of 128, e4m3, rotated): rows in registers, read when their job comes,
-// 79 us; with the copies ahead, pairs of values per instruction and whole runs of addresses per piece 74 us (51 us
-// without the rotation, whose angles come from the L1 cache twice for every head; 38 us is what the bytes take).
 __device__ __forceinline__ float max_or_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -234,7 +225,16 @@ __device__ __forceinline__ uint4 load_shared_16(uint32_t addr) {
 template <int PASSES>
 constexpr uint32_t kStageBytes = PASSES * 2 * 32 * 16; // one job's rows of a warp
 
-// The rows of one job in shared memory: [row group][piece][lane], 16 bytes each.
+// The usual way: up to PASSES row groups of the warp are copied to its own corner of shared memory while the job before
+// is worked on, and are gone through there twice, for the maximum and for the codes.  (K is rotated both times: the
+// rotated rows as fp32 in registers cost the SM a third of its warps.)  Every lane reads back what it copied itself, so
+// nothing but its own copies has to be waited for.  The maximum of V is taken two fp16 values at a time.  The
+// maxima propagate NaNs, so an infinity or a NaN among the inputs shows in the result.  A lane without a row of its
+// own in a group takes the last row over again: it changes no maximum and is not stored.
+// Measured on 37 376 prompt tokens (8 KV heads of 128, e4m3, rotated): rows in registers, read when their job comes,
+// 79 us; with the copies ahead, pairs of values per instruction and whole runs of addresses per piece 74 us (51 us
+// without the rotation, whose angles come from the L1 cache twice for every head; 38 us is what the bytes take).
+// Layout: [row group][piece][lane], 16 bytes each.
 template <int PASSES, bool ROTATE, bool INTERLEAVED>
 struct HeldRows {
   const RowJob &job;

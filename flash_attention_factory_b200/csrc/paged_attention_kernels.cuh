@@ -804,6 +804,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
             // copies into the slots beside the stage, whose barrier every lane arrives on when its own have
             // landed.  (Fetching them into registers before the stage is armed held every batch of copies
             // back by a trip to memory: 128 sequences up to 8192 tokens of int8, 169 us instead of 158.)
+            __syncwarp(); // lane 0 has seen the stage empty; the other lanes' copies come behind that
             if (valid && lane_chunk / chunks_per_stage == sb) {
               // a block id beyond the cache reads zeros through the descriptor; its scales come from the last block
               const size_t si = static_cast<size_t>(min(block_id, args.num_blocks - 1u)) * args.num_kv_heads +

@@ -256,3 +256,53 @@ def test_decode_steps_with_attention(cuda_device, cache):
         check(out, want, tol, f"step {step}")
         turned, size = rotated64(c["q"][now], c["table"], ctx.long() - 1, False)
         assert ((qo.cpu().double() - turned).abs() <= half_step(turned, size, "fp16", 1.0)).all()
+
+
+@pytest.mark.parametrize("seqs", [31, 32, 33, 500, 1000])
+def test_many_sequences(cuda_device, seqs):
+    """The search for a token's sequence: 31 is the last count that needs no memory, sequences without tokens among them."""
+    g = torch.Generator().manual_seed(seqs)
+    old = torch.randint(0, 40, (seqs,), generator=g).tolist()
+    new = torch.randint(0, 4, (seqs,), generator=g).tolist()
+    new[0], new[-1] = 0, 0
+    c = make(seqs, old, new, 1, 16, 16, "int8", extra_rows=3)
+    compare(run(c, cuda_device), reference(c))
+
+
+def test_nothing_to_append(cuda_device):
+    """No rows, and sequences of which none has a new token: caches and scales stay."""
+    for rows in (0, 4):
+        c = make(3, [5, 9], [0, 0], 2, 64, 16, "e4m3", extra_rows=rows)
+        compare(run(c, cuda_device), reference(c))
+
+
+def test_torch_ops_of_a_step(cuda_device):
+    """The registered operators run a decode step: append with rotation, then attention; rope_and_cache and diff too."""
+    import flash_attention_factory_b200.torch_ops  # noqa: F401
+    from flash_attention_factory_b200.lib import paged_attention_diff
+
+    dev = cuda_device
+    c = make(21, [33, 7], [1, 1], 4, 64, 16, "int8", 64, 8, one_each=True)
+    x = {n: c[n].to(dev).contiguous() for n in ("q", "k", "v", "kc", "vc", "ks", "vs", "bt", "ctx", "table")}
+    qo = torch.empty_like(x["q"])
+    ops = torch.ops.paged_attention_b200
+    ops.append_block_scaled(x["k"], x["v"], x["kc"], x["vc"], x["ks"], x["vs"], x["bt"], x["ctx"], None, x["q"], qo, x["table"])
+    torch.cuda.synchronize(dev)
+    compare([x["kc"].cpu(), x["vc"].cpu(), x["ks"].cpu(), x["vs"].cpu(), qo.cpu()], reference(c))
+    lam = torch.full((4,), 0.4, device=dev)
+    out = [torch.empty(2, 4, 128, dtype=torch.float16, device=dev) for _ in range(2)]
+    args = (qo, x["kc"], x["vc"], x["bt"], x["ctx"], lam, 0.125, 1.0, 16, 34)
+    sc = paged_attention_diff.scratch(qo, x["kc"], 34)
+    ops.diff(*sc, out[0], *args, k_scale_per_block=x["ks"], v_scale_per_block=x["vs"])
+    paged_attention_diff.enqueue(*sc, out[1], *args, k_scale_per_block=x["ks"], v_scale_per_block=x["vs"])
+    assert torch.equal(out[0], out[1])
+    from flash_attention_factory_b200 import cache_ops
+
+    slots = torch.tensor([3, 40], device=dev)
+    pos = torch.tensor([9, 100], device=dev)
+    sides = []
+    for fn in (ops.rope_and_cache, cache_ops.rope_and_cache):
+        kc, vc, q = torch.zeros(4, 16, 4, 64, dtype=torch.float16, device=dev), torch.zeros(4, 16, 4, 64, dtype=torch.float16, device=dev), torch.empty_like(qo)
+        fn(x["q"], x["k"], x["v"], pos, x["table"], q, kc, vc, slots)
+        sides.append((kc, vc, q))
+    assert all(torch.equal(a, b) for a, b in zip(*sides)) and int(sides[0][0].count_nonzero()) > 0

@@ -186,3 +186,42 @@ def test_runs_are_bit_identical_and_overlap(cuda_device):
         assert torch.equal(out.cpu(), once)
     us = go(*sets[0], fn=diff.run)
     assert len(us) == 2 and all(t > 0 for t in us) and torch.equal(sets[0][1].cpu(), once)
+
+
+def test_empty_batch_and_wide_groups_of_pairs(cuda_device):
+    """No sequences at all; 16 KV heads (4 head groups) with the largest group."""
+    from flash_attention_factory_b200.lib import paged_attention_diff as diff
+
+    dev = cuda_device
+    q = torch.empty(0, 8, 64, dtype=torch.float16, device=dev)
+    kc = torch.zeros(2, 16, 4, 64, dtype=torch.float16, device=dev)
+    diff.enqueue(*diff.scratch(q, kc, 0), torch.empty(0, 4, 128, dtype=torch.float16, device=dev), q, kc, kc,
+                 torch.empty(0, 1, dtype=torch.int32, device=dev), torch.empty(0, dtype=torch.int32, device=dev),
+                 torch.ones(4, device=dev), 0.1, 1.0, 16, 0)
+    case = paged_case(30, [333, 1, 90], 128, 16, 64, 64, cache="e5m2", scale="block", spread=4.0)
+    lam, w = learned(64, 64)
+    check(run(case, dev, lam, norm_weight=w), *reference(case, lam, w), "16 KV heads")
+
+
+def test_decode_step_after_the_rotating_append(cuda_device):
+    """rope_and_cache fills the pairs' cache like any other: append, then differential attention over it."""
+    from flash_attention_factory_b200.cache_ops import rope_and_cache
+    from test_rope_cache_gpu import rotated64, table
+
+    dev = cuda_device
+    lens = [40, 7, 130]
+    case = paged_case(31, lens, 8, 4, 64, 16, cache="fp16")
+    g = torch.Generator().manual_seed(2)
+    k, v = (torch.randn(3, 4, 64, generator=g).half() for _ in range(2))
+    pos = torch.tensor(lens) - 1
+    slots = torch.tensor([int(case["block_tables"][i, p // 16]) * 16 + p % 16 for i, p in enumerate(pos.tolist())])
+    c = to(case, dev)
+    qo = torch.empty_like(c["query"])
+    rope_and_cache(c["query"], k.to(dev), v.to(dev), pos.to(dev), table(200, 64).to(dev), qo, c["key_cache"], c["value_cache"], slots.to(dev))
+    torch.cuda.synchronize(dev)
+    turned, size = rotated64(k, table(200, 64), pos, False)
+    held = c["key_cache"].cpu().flatten(0, 1)[slots].double()
+    assert ((held - turned).abs() <= HALF * turned.abs() + 2.0 ** -25 + 4 * 2.0 ** -24 * size).all()
+    after = dict(case, query=qo.cpu(), key_cache=c["key_cache"].cpu(), value_cache=c["value_cache"].cpu())
+    lam, w = learned(4, 64)
+    check(run(after, dev, lam, norm_weight=w), *reference(after, lam, w), "after the append")

@@ -169,3 +169,91 @@ def test_writer_stores_rounded_integers(cuda_device, scales):
                       float(s) if scales == "scalar" else 1.0, **kw)
     torch.cuda.synchronize(cuda_device)
     assert torch.equal(dk.cpu(), want[0]) and torch.equal(dv.cpu(), want[1])
+
+
+@pytest.mark.parametrize("hk,group", [(4, 2), (1, 3)])
+def test_many_short_sequences_run_the_persistent_form(cuda_device, hk, group):
+    """At least four units per SM and a known, short maximum: whole-context items, with a warp per head and with
+    warps that share one, empty contexts among them."""
+    g = torch.Generator().manual_seed(1)
+    lens = torch.randint(0, 90, (700,), generator=g).tolist()
+    case = paged_case(14, lens, hk * group, hk, 64, 16, spread=6.0)
+    want, tol = attention64(case, case["k_scale"], case["v_scale"])
+    check(_run("loop", case, cuda_device, **_scales(case, "block")), want, tol, f"hk{hk}")
+
+
+def test_host_batch_step(cuda_device):
+    """The pipelined host-buffer step takes the int8 entry points; cut into sub-batches it gives the same bits."""
+    from flash_attention_factory_b200 import _cabi
+
+    lens = [700, 40, 1500, 9, 300, 0, 513, 77]
+    case = paged_case(15, lens, 8, 4, 128, 16)
+    direct = _run("reduce", case, cuda_device, **_scales(case, "block"))
+    c = to(case, cuda_device)
+    ml, es = (torch.empty(8, 8, 3, device=cuda_device) for _ in range(2))
+    tmp = torch.empty(8, 8, 3, 128, dtype=torch.float16, device=cuda_device)
+    out = torch.zeros(8, 8, 128, dtype=torch.float16, device=cuda_device)
+    q, bt, cl = (torch.empty_like(c[n]) for n in ("query", "block_tables", "context_lens"))
+    from flash_attention_factory_b200.lib import paged_attention_int8_reduce as mod
+
+    p = mod.params(ml, es, tmp, out, None, q, c["key_cache"], c["value_cache"], bt, cl, 2, case["sm_scale"], 1.0, 16, 1500,
+                   torch.ones(8, device=cuda_device), None, -1.0, **{k: v.to(cuda_device) for k, v in _scales(c, "block").items()})
+    host = [case[n].pin_memory() for n in ("query", "block_tables", "context_lens")]
+    for n in (1, 3):
+        host_out = torch.zeros(8, 8, 128, dtype=torch.float16).pin_memory()
+        io = _cabi.PaHostBatch()
+        io.host_query, io.host_block_tables, io.host_context_lens = (t.data_ptr() for t in host)
+        io.host_out, io.sub_batches = host_out.data_ptr(), n
+        import ctypes
+
+        _cabi.check(_cabi.load_library().pa_decode_step_host_batch(
+            _cabi.ENTRY_IDS[mod.ENTRY], ctypes.byref(p), ctypes.byref(io),
+            ctypes.c_void_p(torch.cuda.current_stream(cuda_device).cuda_stream), 1))
+        assert torch.equal(host_out, direct), n
+
+
+def test_overlapping_and_captured_launches(cuda_device):
+    """Two streams with scratch of their own and a captured, replayed launch, bit for bit against a solitary one."""
+    from flash_attention_factory_b200.lib import paged_attention_int8_reduce as mod
+
+    dev = cuda_device
+    case = paged_case(16, [900] * 40, 16, 8, 128, 16, spread=3.0)
+    once = _run("reduce", case, dev, **_scales(case, "block"))
+    c = to(case, dev)
+    alibi = torch.ones(16, device=dev)
+    sets = [(torch.empty(40, 16, 2, device=dev), torch.empty(40, 16, 2, device=dev),
+             torch.empty(40, 16, 2, 128, dtype=torch.float16, device=dev), torch.empty(40, 16, 128, dtype=torch.float16, device=dev))
+            for _ in range(3)]
+
+    def go(s):
+        mod.enqueue(*s, None, c["query"], c["key_cache"], c["value_cache"], c["block_tables"], c["context_lens"], 2,
+                    case["sm_scale"], 1.0, 16, 900, alibi, None, -1.0, k_scale_per_block=c["k_scale"], v_scale_per_block=c["v_scale"])
+
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    torch.cuda.synchronize(dev)
+    for _ in range(6):
+        for st, s in zip(streams, sets):
+            with torch.cuda.stream(st):
+                go(s)
+    torch.cuda.synchronize(dev)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        go(sets[2])
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize(dev)
+    for s in sets:
+        assert torch.equal(s[3].cpu(), once)
+
+
+def test_block_ids_outside_the_cache_read_zeros(cuda_device):
+    """As in the FP8 operators: such a block is zeros (under the scale of the last block)."""
+    case = paged_case(17, [40], 4, 4, 64, 16)
+    zeroed = {k: (v.clone() if torch.is_tensor(v) else v) for k, v in case.items()}
+    block = int(case["block_tables"][0, 1])
+    zeroed["key_cache"][block] = 0
+    zeroed["value_cache"][block] = 0
+    want, tol = attention64(zeroed, case["k_scale"], case["v_scale"])
+    case["block_tables"][0, 1] = case["key_cache"].size(0) + 7
+    for variant in ("loop", "reduce"):
+        check(_run(variant, case, cuda_device, **_scales(case, "block")), want, tol, variant)
