@@ -17,7 +17,7 @@ import torch
 
 from . import _cabi, _launch
 
-_F16 = torch.float16
+_F16, _F32, _I64 = torch.float16, torch.float32, torch.int64
 
 
 def _kv_dtype(cache: torch.Tensor) -> int:
@@ -32,18 +32,23 @@ def _kv_dtype(cache: torch.Tensor) -> int:
     raise RuntimeError(f"unsupported cache dtype {cache.dtype}")
 
 
-def _set_scales(p, key, key_cache, k_scale_per_head, v_scale_per_head, k_scale_per_block, v_scale_per_block) -> None:
-    per_head, per_block = (key.size(1),), (key_cache.size(0), key.size(1))
-    for name, t, shape in (("k_scale_per_head", k_scale_per_head, per_head),
-                           ("v_scale_per_head", v_scale_per_head, per_head),
-                           ("k_scale_per_block", k_scale_per_block, per_block),
-                           ("v_scale_per_block", v_scale_per_block, per_block)):
-        if t is None:
-            continue
-        if (t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous()
-                or t.device != key.device):
-            raise RuntimeError(f"{name} must be a contiguous float32 tensor of shape {shape} on the cache's device")
-        setattr(p, name, t.data_ptr())
+def _set_scales(p, num_blocks: int, kv_heads: int, index: int, k_scale_per_head, v_scale_per_head, k_scale_per_block,
+                v_scale_per_block) -> None:
+    """Fills the scale arrays of a cache-write argument block from those that are given."""
+    if k_scale_per_head is not None:
+        p.k_scale_per_head = _scale_pointer(k_scale_per_head, "k_scale_per_head", (kv_heads,), index)
+    if v_scale_per_head is not None:
+        p.v_scale_per_head = _scale_pointer(v_scale_per_head, "v_scale_per_head", (kv_heads,), index)
+    if k_scale_per_block is not None:
+        p.k_scale_per_block = _scale_pointer(k_scale_per_block, "k_scale_per_block", (num_blocks, kv_heads), index)
+    if v_scale_per_block is not None:
+        p.v_scale_per_block = _scale_pointer(v_scale_per_block, "v_scale_per_block", (num_blocks, kv_heads), index)
+
+
+def _scale_pointer(t: torch.Tensor, name: str, shape, index: int) -> int:
+    if t.dtype is not _F32 or t.shape != shape or t.get_device() != index or not t.is_contiguous():
+        raise RuntimeError(f"{name} must be a contiguous float32 tensor of shape {shape} on the cache's device")
+    return t.data_ptr()
 
 
 def reshape_and_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor,
@@ -79,57 +84,56 @@ def reshape_and_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.T
     p.block_size, p.num_blocks = key_cache.size(1), key_cache.size(0)
     p.fp8_scale = float(fp8_scale)
     p.kv_dtype = _kv_dtype(key_cache)
-    _set_scales(p, key, key_cache, k_scale_per_head, v_scale_per_head, k_scale_per_block, v_scale_per_block)
+    _set_scales(p, key_cache.size(0), key.size(1), key.get_device(), k_scale_per_head, v_scale_per_head,
+                k_scale_per_block, v_scale_per_block)
     lib = _cabi.load_library()
     with torch.cuda.device(key.device):
         stream = torch.cuda.current_stream(key.device).cuda_stream
         _cabi.check(lib.pa_reshape_and_cache(ctypes.byref(p), ctypes.c_void_p(stream)))
 
 
-def _token_rows(t: torch.Tensor, name: str, index: int) -> int:
+def _token_rows(t: torch.Tensor, shape, name: str, index: int) -> int:
     """Checks fp16 rows [T, heads, D] whose tokens may lie any stride apart (slices of one projection's
     output); returns that stride in elements."""
-    if t.dtype is not _F16 or t.dim() != 3 or t.get_device() != index:
+    if t.dtype is not _F16 or len(shape) != 3 or t.get_device() != index:
         raise RuntimeError(f"{name} must be a float16 tensor [tokens, heads, head_size] on the cache's device")
-    tokens, heads, d = t.shape
+    tokens, heads, d = shape
     stride, head_stride, last = t.stride()
-    if last != 1 or (heads != 1 and head_stride != d):
+    if last != 1 or (head_stride != d and heads != 1):
         raise RuntimeError(f"the heads of a token of {name} must be contiguous")
     if tokens <= 1:
         return heads * d
-    if stride < 0 or stride % 8 != 0:
+    if stride % 8 != 0 or stride < 0:
         raise RuntimeError(f"the token stride of {name} must be a multiple of 8 elements")
     return stride
 
 
-def _check_caches(key, value, key_cache, value_cache) -> int:
-    """Checks the caches against the rows; returns the device index."""
+def _check_caches(rows, value, key_cache, value_cache, shape) -> int:
+    """Checks the caches (of `shape`) against the rows of key and value; returns the device index."""
     index = key_cache.get_device()
     if index < 0 or value_cache.get_device() != index or not (key_cache.is_contiguous() and value_cache.is_contiguous()):
         raise RuntimeError("the caches must be contiguous CUDA tensors on one device (no CPU fallback exists)")
-    shape = key_cache.shape
     if len(shape) != 4 or shape != value_cache.shape or key_cache.dtype is not value_cache.dtype:
         raise RuntimeError("key_cache and value_cache must match")
-    rows = key.shape
-    if rows != value.shape or shape[2:] != rows[1:]:
+    if len(rows) != 3 or rows != value.shape or rows[1] != shape[2] or rows[2] != shape[3]:
         raise RuntimeError("cache must be [num_blocks, block_size, num_kv_heads, head_size]")
     return index
 
 
 def _check_rotation(cos_sin, index: int) -> None:
-    if (cos_sin.dtype is not torch.float32 or cos_sin.dim() != 2 or not cos_sin.is_contiguous()
+    if (cos_sin.dtype is not _F32 or cos_sin.dim() != 2 or not cos_sin.is_contiguous()
             or cos_sin.get_device() != index):
         raise RuntimeError("cos_sin must be a contiguous float32 tensor [max_position, rotary_dim] on the cache's device")
 
 
-def _check_queries(p, query, query_out, key, index: int) -> None:
+def _check_queries(p, query, query_out, rows, index: int) -> None:
     """Fills the query part of an argument block."""
     if query is None and query_out is None:
         return
     if query is None or query_out is None:
         raise RuntimeError("query and query_out must be given together")
-    p.query_token_stride = _token_rows(query, "query", index)
-    shape, rows = query.shape, key.shape
+    shape = query.shape
+    p.query_token_stride = _token_rows(query, shape, "query", index)
     if shape[0] != rows[0] or shape[2] != rows[2]:
         raise RuntimeError("query and key must have the same tokens and head_size")
     if (query_out.shape != shape or query_out.dtype is not _F16 or not query_out.is_contiguous()
@@ -155,17 +159,18 @@ def rope_and_cache(query, key: torch.Tensor, value: torch.Tensor, positions: tor
     or whose slot or position is out of range, is skipped: its cache and query_out rows stay as they
     were.  Asynchronous on torch's current stream.
     """
-    index = _check_caches(key, value, key_cache, value_cache)
+    shape, rows = key_cache.shape, key.shape
+    index = _check_caches(rows, value, key_cache, value_cache, shape)
     p = _cabi.PaRopeCacheParams()
-    p.key_token_stride = _token_rows(key, "key", index)
-    p.value_token_stride = _token_rows(value, "value", index)
-    num_blocks, block_size, kv_heads, head_size = key_cache.shape
-    tokens = key.shape[0]
+    p.key_token_stride = _token_rows(key, rows, "key", index)
+    p.value_token_stride = _token_rows(value, rows, "value", index)
+    num_blocks, block_size, kv_heads, head_size = shape
+    tokens = rows[0]
     for x in (slot_mapping, positions):
-        if x.dtype is not torch.int64 or x.numel() != tokens or not x.is_contiguous() or x.get_device() != index:
+        if x.dtype is not _I64 or x.numel() != tokens or not x.is_contiguous() or x.get_device() != index:
             raise RuntimeError("slot_mapping and positions must be int64 with one entry per token on the cache's device")
     _check_rotation(cos_sin, index)
-    _check_queries(p, query, query_out, key, index)
+    _check_queries(p, query, query_out, rows, index)
     c = p.cache
     c.key, c.value = key.data_ptr(), value.data_ptr()
     c.key_cache, c.value_cache = key_cache.data_ptr(), value_cache.data_ptr()
@@ -174,7 +179,7 @@ def rope_and_cache(query, key: torch.Tensor, value: torch.Tensor, positions: tor
     c.block_size, c.num_blocks = block_size, num_blocks
     c.fp8_scale, c.kv_dtype = float(fp8_scale), _kv_dtype(key_cache)
     if not (k_scale_per_head is v_scale_per_head is k_scale_per_block is v_scale_per_block is None):
-        _set_scales(c, key, key_cache, k_scale_per_head, v_scale_per_head, k_scale_per_block, v_scale_per_block)
+        _set_scales(c, num_blocks, kv_heads, index, k_scale_per_head, v_scale_per_head, k_scale_per_block, v_scale_per_block)
     p.positions, p.cos_sin = positions.data_ptr(), cos_sin.data_ptr()
     p.max_position, p.rotary_dim = cos_sin.shape
     p.interleaved = int(interleaved)
@@ -200,13 +205,14 @@ def append_block_scaled(key: torch.Tensor, value: torch.Tensor, key_cache: torch
     behind the last sequence, and tokens whose position lies outside the table row or the rotation table, are
     skipped.  Asynchronous on torch's current stream.
     """
-    index = _check_caches(key, value, key_cache, value_cache)
+    shape, rows = key_cache.shape, key.shape
+    index = _check_caches(rows, value, key_cache, value_cache, shape)
     p = _cabi.PaBlockScaledParams()
-    p.key_token_stride = _token_rows(key, "key", index)
-    p.value_token_stride = _token_rows(value, "value", index)
-    num_blocks, block_size, kv_heads, head_size = key_cache.shape
+    p.key_token_stride = _token_rows(key, rows, "key", index)
+    p.value_token_stride = _token_rows(value, rows, "value", index)
+    num_blocks, block_size, kv_heads, head_size = shape
     for t in (k_scale_per_block, v_scale_per_block):
-        if (t.dtype is not torch.float32 or t.shape != (num_blocks, kv_heads) or not t.is_contiguous()
+        if (t.dtype is not _F32 or t.shape != (num_blocks, kv_heads) or not t.is_contiguous()
                 or t.get_device() != index):
             raise RuntimeError("k_scale_per_block and v_scale_per_block must be contiguous float32 tensors "
                                "[num_blocks, num_kv_heads] on the cache's device")
@@ -226,12 +232,12 @@ def append_block_scaled(key: torch.Tensor, value: torch.Tensor, key_cache: torch
         p.max_position, p.rotary_dim = cos_sin.shape
     elif query is not None:
         raise RuntimeError("queries are only taken to be rotated: cos_sin is missing")
-    _check_queries(p, query, query_out, key, index)
+    _check_queries(p, query, query_out, rows, index)
     p.key, p.value = key.data_ptr(), value.data_ptr()
     p.key_cache, p.value_cache = key_cache.data_ptr(), value_cache.data_ptr()
     p.k_scale_per_block, p.v_scale_per_block = k_scale_per_block.data_ptr(), v_scale_per_block.data_ptr()
     p.block_tables, p.context_lens = block_tables.data_ptr(), context_lens.data_ptr()
-    p.num_seqs, p.num_tokens, p.num_kv_heads, p.head_size = seqs, key.shape[0], kv_heads, head_size
+    p.num_seqs, p.num_tokens, p.num_kv_heads, p.head_size = seqs, rows[0], kv_heads, head_size
     p.block_size, p.max_blocks_per_seq, p.num_blocks = block_size, block_tables.shape[1], num_blocks
     p.kv_dtype, p.interleaved = _kv_dtype(key_cache), int(interleaved)
     _launch.call(_cabi.load_library().pa_append_block_scaled, p, index)

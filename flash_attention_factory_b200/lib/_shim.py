@@ -36,6 +36,14 @@ def _kv_dtype_of(cache: torch.Tensor, fp8: bool, int8: bool = False) -> int:
     return _cabi.KV_FP8_E5M2
 
 
+def _block_scale(t: torch.Tensor, name: str, shape, index: int, fp8: bool) -> int:
+    if not fp8:
+        raise RuntimeError("per-block scales belong to the FP8 and int8 operators")
+    if t.dtype is not _F32 or t.shape != shape or t.get_device() != index or not t.is_contiguous():
+        raise RuntimeError(f"{name} must be float32 [num_blocks, num_kv_heads] on the device")
+    return t.data_ptr()
+
+
 def build_params(max_logits, exp_sums, tem_output, output, debug_output, query, key_cache,
                  value_cache, block_tables, context_lens, num_queries_per_tokens, sm_scale,
                  fp8_scale, block_size, max_context_len, alibi_slopes, sinks, softcap,
@@ -117,15 +125,10 @@ def build_params(max_logits, exp_sums, tem_output, output, debug_output, query, 
                 _require(t.dtype == torch.float32 and t.is_contiguous() and t.device == query.device
                          and t.numel() == kv_heads, f"{name} must be float32 [num_kv_heads] on the device")
                 setattr(p, name, t.data_ptr())
-    if k_scale_per_block is not None or v_scale_per_block is not None:
-        for name, t in (("k_scale_per_block", k_scale_per_block), ("v_scale_per_block", v_scale_per_block)):
-            if t is not None:
-                if not fp8:
-                    raise RuntimeError("per-block scales belong to the FP8 and int8 operators")
-                if (t.dtype is not _F32 or not t.is_contiguous() or t.get_device() != index
-                        or t.shape != (num_blocks, kv_heads)):
-                    raise RuntimeError(f"{name} must be float32 [num_blocks, num_kv_heads] on the device")
-                setattr(p, name, t.data_ptr())
+    if k_scale_per_block is not None:
+        p.k_scale_per_block = _block_scale(k_scale_per_block, "k_scale_per_block", (num_blocks, kv_heads), index, fp8)
+    if v_scale_per_block is not None:
+        p.v_scale_per_block = _block_scale(v_scale_per_block, "v_scale_per_block", (num_blocks, kv_heads), index, fp8)
     # opt-in only: by default alibi_slopes and softcap are ignored, as in the reference
     if use_alibi:
         _require(alibi_slopes.is_cuda and alibi_slopes.is_contiguous()
