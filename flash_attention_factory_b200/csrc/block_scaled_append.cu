@@ -93,6 +93,7 @@ __device__ __forceinline__ TokenPlace place_token(const AppendArgs &a, uint32_t 
 
 constexpr uint32_t kAppendThreads = 256;
 constexpr uint32_t kAppendWarps = kAppendThreads / 32;
+constexpr uint32_t kQueryBatch = 4; // query rows that a thread requests together
 
 // What a lane does of every row group: the lanes of a warp hold rows_per_pass rows side by side, 16 elements
 // each (see rotary_item).
@@ -457,25 +458,39 @@ __global__ void __launch_bounds__(kAppendThreads, 3) append_block_scaled_kernel(
   const RotaryItem rot = rotary_item(item, a.rotary_dim, INTERLEAVED);
   const uint32_t pairs = a.tokens_per_cta * a.num_heads;
   const uint32_t step = (gridDim.y - a.append_ctas) * pairs_at_once;
-#pragma unroll 2
-  for (uint32_t p0 = (blockIdx.y - a.append_ctas) * pairs_at_once; p0 < pairs; p0 += step) { // the same trips for all lanes: they shuffle
-    const uint32_t pair = p0 + pair0;
-    const uint32_t t = pair / a.num_heads, head = pair - t * a.num_heads;
-    const uint32_t position = __shfl_sync(0xffffffffu, mine.position, t & 31u);
-    const bool valid = __shfl_sync(0xffffffffu, mine.valid ? 1 : 0, t & 31u) != 0;
-    if (pair0 >= pairs_at_once || pair >= pairs || !valid) continue;
-    const __half *row = a.query + static_cast<size_t>(token0 + t) * a.query_stride + static_cast<size_t>(head) * D;
-    __half *dst = a.query_out + (static_cast<size_t>(token0 + t) * a.num_heads + head) * D;
-    float x[8], y[8];
-    unpack_half8(__ldg(reinterpret_cast<const uint4 *>(row + rot.first)), x);
-    unpack_half8(__ldg(reinterpret_cast<const uint4 *>(row + rot.second)), y);
-    if (rot.rotated) {
-      float c[8], s[8];
-      load_cos_sin(a.cos_sin + static_cast<size_t>(position) * a.rotary_dim, item, a.rotary_dim, c, s);
-      rotate_item(x, y, c, s, INTERLEAVED);
+  for (uint32_t p0 = (blockIdx.y - a.append_ctas) * pairs_at_once; p0 < pairs; p0 += kQueryBatch * step) { // the same trips for all lanes: they shuffle
+    uint4 raw[kQueryBatch][2];
+    uint32_t position[kQueryBatch];
+    size_t row[kQueryBatch]; // token * num_heads + head
+    bool take[kQueryBatch];
+#pragma unroll
+    for (uint32_t k = 0; k < kQueryBatch; ++k) {
+      const uint32_t pair = p0 + k * step + pair0;
+      const uint32_t t = pair / a.num_heads, head = pair - t * a.num_heads;
+      position[k] = __shfl_sync(0xffffffffu, mine.position, t & 31u);
+      take[k] = __shfl_sync(0xffffffffu, mine.valid ? 1 : 0, t & 31u) != 0 && pair0 < pairs_at_once && pair < pairs;
+      row[k] = static_cast<size_t>(token0 + t) * a.num_heads + head;
+      if (take[k]) {
+        const __half *src = a.query + static_cast<size_t>(token0 + t) * a.query_stride + static_cast<size_t>(head) * D;
+        raw[k][0] = __ldg(reinterpret_cast<const uint4 *>(src + rot.first));
+        raw[k][1] = __ldg(reinterpret_cast<const uint4 *>(src + rot.second));
+      }
     }
-    *reinterpret_cast<uint4 *>(dst + rot.first) = pack_half8(x);
-    *reinterpret_cast<uint4 *>(dst + rot.second) = pack_half8(y);
+#pragma unroll
+    for (uint32_t k = 0; k < kQueryBatch; ++k) {
+      if (!take[k]) continue;
+      Item2 v;
+      unpack_item(raw[k][0], raw[k][1], v);
+      if (rot.rotated) {
+        const float *angles = a.cos_sin + static_cast<size_t>(position[k]) * a.rotary_dim + item * 8u;
+        rotate_item2(v, angles, angles + a.rotary_dim / 2u, INTERLEAVED);
+      }
+      __half *dst = a.query_out + row[k] * D;
+      *reinterpret_cast<uint4 *>(dst + rot.first) = make_uint4(pack_half2(v.x[0].x, v.x[0].y), pack_half2(v.x[1].x, v.x[1].y),
+                                                               pack_half2(v.x[2].x, v.x[2].y), pack_half2(v.x[3].x, v.x[3].y));
+      *reinterpret_cast<uint4 *>(dst + rot.second) = make_uint4(pack_half2(v.y[0].x, v.y[0].y), pack_half2(v.y[1].x, v.y[1].y),
+                                                                pack_half2(v.y[2].x, v.y[2].y), pack_half2(v.y[3].x, v.y[3].y));
+    }
   }
 }
 
@@ -570,13 +585,15 @@ extern "C" PA_API int pa_append_block_scaled(const pa_block_scaled_params *p, vo
   uint32_t parts = 1;
   while (parts < kAppendWarps && parts * (few ? 1u : 4u) * rows_per_pass < rows) parts *= 2u;
   a.warps_per_job = parts;
-  // enough CTAs in a column to fill the GPU once or twice, no more than it has work for
+  // CTAs in a column: enough to fill the 444 places of the GPU twice or so, no more than there is work for.  (9 163
+  // tokens of 37 sequences, 8 KV heads of 64, blocks of 64: without queries 19.2 us with 4 CTAs, 24 with 2; with 40
+  // query heads 34.8 us with 2 + 3, 36.8 with 4 + 3, 40 with 4 + 1, 38 with 4 + 6.)
   const uint32_t columns = divide_round_up(p->num_tokens, per_cta);
-  const uint32_t wanted = std::max(1u, 1184u / columns);
-  a.append_ctas = std::min(wanted, divide_round_up(2u * p->num_kv_heads * parts, kAppendWarps));
+  auto ctas = [&](uint32_t aimed_at, uint32_t useful) { return std::min(std::max(1u, aimed_at / columns), useful); };
+  a.append_ctas = ctas(p->query != nullptr ? 592u : 1184u, divide_round_up(2u * p->num_kv_heads * parts, kAppendWarps));
   uint32_t query_ctas = 0;
   if (p->query != nullptr)
-    query_ctas = std::min(wanted, divide_round_up(per_cta * p->num_heads * (p->head_size / 16u), kAppendThreads));
+    query_ctas = ctas(888u, divide_round_up(per_cta * p->num_heads * (p->head_size / 16u), kQueryBatch * kAppendThreads));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool interleaved = p->interleaved != 0u;
   auto launch = [&](auto few_rows, auto many_rows) {
