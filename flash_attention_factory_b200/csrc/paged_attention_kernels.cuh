@@ -571,6 +571,15 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
   // straight-line path too, with a running reference for the V scales (see fold_v_scales); the FP8
   // caches of ordinary attention keep them on the general path, where their order of operations was set.
   constexpr bool BLOCK_FAST = (KV == KV_I8) || (VH == 2 && KV != KV_F16);
+  // Weights in two parts: the value product takes the weight rounded to fp16 and, as a second MMA on the same V
+  // fragment, the rounded rest of it, so that the rounding of the weights no longer shows.  Taken where it is
+  // the largest of the errors: differential attention over an fp16 cache, where the maps' outputs cancel (error
+  // against fp64 3.2e-4 -> 2.1e-4, that of the rounded result itself; 48 sequences up to 8192 tokens 135 -> 139 us), and
+  // the split int8 kernel, whose partial rows are rounded to fp16 as well (3.5e-4 -> 2.9e-4; 152 -> 155 us).
+  // Not for differential attention over 8-bit caches: their codes are off by 2^-8 to 2^-3, and the kernel, which
+  // converts every V code twice, would be 19 % slower (59 -> 70 us on 2 x 65536 tokens of e4m3).
+  constexpr bool TWO_PART_WEIGHTS = (VH == 2 && KV == KV_F16) || (VH == 1 && KV == KV_I8 && MODE == MODE_SPLIT);
+  constexpr uint32_t WP = TWO_PART_WEIGHTS ? 2u : 1u; // parts of a weight
 
   const uint32_t warp = threadIdx.x >> 5;
   const uint32_t lane = threadIdx.x & 31u;
@@ -803,8 +812,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
             // The scales of the stage's (block, head) pairs travel like its tiles: 4-byte asynchronous
             // copies into the slots beside the stage, whose barrier every lane arrives on when its own have
             // landed.  (Fetching them into registers before the stage is armed held every batch of copies
-            // back by a trip to memory: 128 sequences up to 8192 tokens of int8, 169 us instead of 158.)
-            __syncwarp(); // lane 0 has seen the stage empty; the other lanes' copies come behind that
+            // back by a trip to memory: 128 sequences up to 8192 tokens of int8, 169 us instead of 158.)  The
+            // shuffle above has put them behind lane 0's look at the empty barrier, as it has the tile copies; a
+            // further __syncwarp here cost 8 %.
             if (valid && lane_chunk / chunks_per_stage == sb) {
               // a block id beyond the cache reads zeros through the descriptor; its scales come from the last block
               const size_t si = static_cast<size_t>(min(block_id, args.num_blocks - 1u)) * args.num_kv_heads +
@@ -939,14 +949,15 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
       }
     };
     // O^T += V^T . P^T for 16 tokens: V (A operand, transposed load) from shared memory
-    auto value_tile = [&](uint32_t v_base, uint32_t p_lo, uint32_t p_hi, float (&o)[KSTEPS][4]) {
+    auto value_tile = [&](uint32_t v_base, const uint32_t (&p_lo)[WP], const uint32_t (&p_hi)[WP], float (&o)[KSTEPS][4]) {
       if constexpr (KV == KV_F16) {
         const uint32_t v_addr = v_base + lm_off_b;
 #pragma unroll
         for (uint32_t i = 0; i < KSTEPS; ++i) {
           uint32_t a[4];
           ldmatrix_x4_trans(a, (v_addr ^ ((i % PAIRS_PER_SLAB) << 5)) + (i / PAIRS_PER_SLAB) * L::SLAB_TILE);
-          mma_m16n8k16(o[i], a, p_lo, p_hi);
+#pragma unroll
+          for (uint32_t w = 0; w < WP; ++w) mma_m16n8k16(o[i], a, p_lo[w], p_hi[w]);
         }
       } else {
         const uint32_t v_addr = v_base + lm_off_a;
@@ -963,8 +974,11 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
           fp8x4_to_even_odd_half2<KV>(r[2], ae[1], ao[1]);
           fp8x4_to_even_odd_half2<KV>(r[1], ae[2], ao[2]);
           fp8x4_to_even_odd_half2<KV>(r[3], ae[3], ao[3]);
-          mma_m16n8k16(o[2 * qq], ae, p_lo, p_hi);
-          mma_m16n8k16(o[2 * qq + 1], ao, p_lo, p_hi);
+#pragma unroll
+          for (uint32_t w = 0; w < WP; ++w) {
+            mma_m16n8k16(o[2 * qq], ae, p_lo[w], p_hi[w]);
+            mma_m16n8k16(o[2 * qq + 1], ao, p_lo[w], p_hi[w]);
+          }
         }
       }
     };
@@ -1002,7 +1016,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
     const uint32_t v_shift = (v_head0 - my_head) * tps * geo::slab_bytes; // 0, or minus one head (modulo 2^32)
     const uint32_t v_head_bytes = tps * geo::slab_bytes;
     // O^T += V^T . P^T over the VH heads, each with its own weights
-    auto value_tiles = [&](uint32_t v_base, const uint32_t (&p_lo)[VH], const uint32_t (&p_hi)[VH]) {
+    auto value_tiles = [&](uint32_t v_base, const uint32_t (&p_lo)[VH][WP], const uint32_t (&p_hi)[VH][WP]) {
 #pragma unroll
       for (uint32_t vh = 0; vh < VH; ++vh)
         value_tile(v_base + v_shift + vh * v_head_bytes, p_lo[vh], p_hi[vh], acc[vh]);
@@ -1046,21 +1060,32 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
       }
     };
     // fp16 weights of one tile as the B operand of the value product, transposed, one set per V head
-    auto pack_weights = [&](const float (&p)[4], const float (&w)[VH], bool weighted, uint32_t (&lo)[VH],
-                            uint32_t (&hi)[VH]) {
+    auto pack_pair = [&](float p0, float p1, uint32_t (&part)[WP]) {
+      const uint32_t rounded = pack_half2(p0, p1);
+      part[0] = movmatrix_trans(rounded);
+      if constexpr (TWO_PART_WEIGHTS) {
+        const float2 back = __half22float2(*reinterpret_cast<const __half2 *>(&rounded));
+        part[1] = movmatrix_trans(pack_half2(p0 - back.x, p1 - back.y));
+      }
+    };
+    auto pack_weights = [&](const float (&p)[4], const float (&w)[VH], bool weighted, uint32_t (&lo)[VH][WP],
+                            uint32_t (&hi)[VH][WP]) {
       if (!weighted) {
-        lo[0] = movmatrix_trans(pack_half2(p[0], p[1])); // tokens 0..7
-        hi[0] = movmatrix_trans(pack_half2(p[2], p[3])); // tokens 8..15
+        pack_pair(p[0], p[1], lo[0]); // tokens 0..7
+        pack_pair(p[2], p[3], hi[0]); // tokens 8..15
         if constexpr (VH == 2) {
-          lo[1] = lo[0];
-          hi[1] = hi[0];
+#pragma unroll
+          for (uint32_t k = 0; k < WP; ++k) {
+            lo[1][k] = lo[0][k];
+            hi[1][k] = hi[0][k];
+          }
         }
         return;
       }
 #pragma unroll
       for (uint32_t vh = 0; vh < VH; ++vh) {
-        lo[vh] = movmatrix_trans(pack_half2(p[0] * w[vh], p[1] * w[vh]));
-        hi[vh] = movmatrix_trans(pack_half2(p[2] * w[vh], p[3] * w[vh]));
+        pack_pair(p[0] * w[vh], p[1] * w[vh], lo[vh]);
+        pack_pair(p[2] * w[vh], p[3] * w[vh], hi[vh]);
       }
     };
     // K scale (log2-domain softmax scale) and V scales of the tile that starts at `row` of a stage.
@@ -1189,9 +1214,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
           // ---- the common case, two full tiles and no score modifiers, free of branches up
           // to the rescale test; every value is computed as in the general case below
           float ca[4], cb[4];
-          score_tile_pair(base_a + lm_off_a, base_b + lm_off_a, qf, ca, cb);
           float s_a = scale, s_b = scale; // softmax scales of the two tiles
           float w_a[VH], w_b[VH];         // V scales of the two tiles over the reference
+          score_tile_pair(base_a + lm_off_a, base_b + lm_off_a, qf, ca, cb);
           if constexpr (BLOCK_FAST) {
             if (block_scales) {
               float v_a[VH], v_b[VH];
@@ -1224,7 +1249,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
           }
           l_run[0] += (pa[0] + pa[2]) + (pb[0] + pb[2]);
           l_run[1] += (pa[1] + pa[3]) + (pb[1] + pb[3]);
-          uint32_t pa_lo[VH], pa_hi[VH], pb_lo[VH], pb_hi[VH];
+          uint32_t pa_lo[VH][WP], pa_hi[VH][WP], pb_lo[VH][WP], pb_hi[VH][WP];
           const bool weighted = BLOCK_FAST && block_scales;
           pack_weights(pa, w_a, weighted, pa_lo, pa_hi);
           pack_weights(pb, w_b, weighted, pb_lo, pb_hi);
@@ -1349,7 +1374,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
           // P rounded to fp16 for the MMA, transposed into the B-operand layout;
           // ---- O^T += V^T . P^T
           {
-            uint32_t p_lo[VH], p_hi[VH];
+            uint32_t p_lo[VH][WP], p_hi[VH][WP];
             pack_weights(pa, w_a, weighted, p_lo, p_hi);
             value_tiles(base_a + L::KV_TILE, p_lo, p_hi);
           }
@@ -1360,7 +1385,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
             released_a = true;
           }
           if (act_b) {
-            uint32_t p_lo[VH], p_hi[VH];
+            uint32_t p_lo[VH][WP], p_hi[VH][WP];
             pack_weights(pb, w_b, weighted, p_lo, p_hi);
             value_tiles(base_b + L::KV_TILE, p_lo, p_hi);
           }
