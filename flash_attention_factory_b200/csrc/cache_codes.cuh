@@ -51,7 +51,7 @@ __device__ __forceinline__ void unpack_codes(uint32_t v, float (&x)[4]) {
 // processor", 1990), q + (x - q s) r, gives the correctly rounded quotient but for rare cases of one unit,
 // so a code can differ from that of the rounded quotient only where the quotient lies within 2^-23 of
 // itself from a rounding border.  Three operations instead of a full division.  The residual needs s and 1 / s away from the ends
-// of the exponent range; other scales take the division.
+// of the exponent range; other scales take the division.  So do infinities, whose residual is a NaN.
 struct Divider {
   float s, r;
   bool plain;
@@ -68,7 +68,10 @@ struct Divider {
 
 // Eight values over their scale
 __device__ __forceinline__ void divide8(float (&x)[8], const Divider &by) {
-  if (by.plain) {
+  float largest = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) largest = fmaxf(largest, fabsf(x[j])); // passes over NaNs, which stay NaNs either way
+  if (by.plain || largest > 3.0e38f) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = __fdiv_rn(x[j], by.s);
   } else {

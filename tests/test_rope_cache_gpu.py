@@ -125,6 +125,27 @@ def test_skipped_tokens_leave_their_rows(cuda_device):
     verify(c, *call(c, cuda_device, False), False, skipped=(4, 7, 8, 10, 11, 12, 49))
 
 
+@pytest.mark.parametrize("cache,largest", [("int8", 127.0), ("e4m3", 448.0), ("e5m2", 57344.0)])
+@pytest.mark.parametrize("scales", ["scalar", "head", "block"])
+def test_infinities_saturate(cuda_device, cache, largest, scales):
+    """An infinity over a finite scale is an infinity, and a cache stores that as its largest code, in V, in the
+    unrotated and in the rotated dims of K (a' = inf cos, b' = inf sin); the values beside it are as ever."""
+    c = case(11, 9, 2, 2, 64, 32, 16, cache, scales, strided=False)
+    clean = call(c, cuda_device, False)
+    inf = float("inf")
+    c["positions"][:] = 1  # cos and sin of every angle are positive
+    c["v"][3, 1, 7], c["v"][3, 1, 8], c["v"][4, 0, 63] = inf, -inf, inf
+    c["k"][5, 0, 40], c["k"][6, 1, 33] = -inf, inf
+    c["k"][7, 1, 2] = inf
+    _, kc, vc = call(c, cuda_device, False)
+    k, v = (cache_values(x.cpu().view(1, -1, 2, 64))[0][c["slots"]] for x in (kc, vc))
+    before = cache_values(clean[2].cpu().view(1, -1, 2, 64))[0][c["slots"]]
+    assert [v[3, 1, 7], v[3, 1, 8], v[4, 0, 63]] == [largest, -largest, largest]
+    assert [k[5, 0, 40], k[6, 1, 33], k[7, 1, 2], k[7, 1, 18]] == [-largest, largest, largest, largest]
+    same = c["v"].isfinite()
+    assert torch.equal(v[same], before[same])
+
+
 def test_without_queries_and_in_place(cuda_device):
     c = case(4, 33, 4, 2, 128, 128, 16, "fp16", "none", strided=False)
     out, kc, vc = call(c, cuda_device, False, queries=False)
