@@ -1048,10 +1048,11 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
       float top = fmaxf(va[0], vb[0]);
       if constexpr (VH == 2) top = fmaxf(top, fmaxf(va[1], vb[1]));
       if (top > v_ref) {
-        const float r = v_ref / top;
+        const float next = fmaxf(top, 0x1p-126f); // the reciprocal of a subnormal scale would be infinite
+        const float r = v_ref / next;
         scale_accumulators(r, r);
-        v_ref = top;
-        v_inv = 1.f / top;
+        v_ref = next;
+        v_inv = 1.f / next;
       }
 #pragma unroll
       for (uint32_t vh = 0; vh < VH; ++vh) {

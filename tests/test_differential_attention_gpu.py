@@ -116,6 +116,13 @@ def test_garbage_behind_the_context(cuda_device):
     check(run(case, cuda_device, lam), *want, "garbage")
 
 
+def test_subnormal_value_scales(cuda_device):
+    """Block scales whose reciprocal is infinite: the result is below every fp16 number."""
+    case = paged_case(7, [300, 20], 8, 4, 64, 16, cache="e4m3", scale="block")
+    case["v_scale"][:] = 1e-40
+    assert (run(case, cuda_device, torch.full((4,), 0.5)) == 0).all()
+
+
 def test_equal_maps_and_weight_one_cancel(cuda_device):
     """Both maps equal and lambda 1: the difference is a rounding of the partial sums, the norm keeps it finite."""
     case = paged_case(6, [300, 17], 4, 2, 64, 16, cache="fp16")

@@ -85,6 +85,18 @@ def test_values_of_very_different_size(cuda_device, variant):
     assert float(want.abs().max()) < 1e-3
 
 
+@pytest.mark.parametrize("variant", ["loop", "reduce"])
+def test_subnormal_value_scales(cuda_device, variant):
+    """Scales whose reciprocal is infinite, alone (the result is below every fp16 number) and beside ordinary ones."""
+    case = paged_case(14, [300, 20], 4, 2, 64, 16)
+    case["v_scale"][:] = 1e-40
+    assert (_run(variant, case, cuda_device, **_scales(case, "block")) == 0).all()
+    case = paged_case(14, [300, 20], 4, 2, 64, 16)
+    case["v_scale"][::2] = 1e-40
+    want, tol = attention64(case, case["k_scale"], case["v_scale"])
+    check(_run(variant, case, cuda_device, **_scales(case, "block")), want, tol, variant)
+
+
 def test_scales_of_blocks_outside_the_context_are_not_used(cuda_device):
     case = paged_case(10, [40, 16], 4, 2, 128, 16)
     used = {int(b) for i, n in enumerate([40, 16]) for b in case["block_tables"][i, : -(-n // 16)]}
