@@ -7,8 +7,9 @@
 //   rows held before:  code' = round(code * s / s')   (only where s' > s)
 //   new rows:          code  = round(x / s')
 // x is the fp32 value of the row, rotated on the way if the call asks for it (see rope_cache.cu).
-// Bound by HBM on prompts (every new element is read once from memory and its code written once)
-// and by latency on decode steps: context length -> block id -> scale and rows -> codes.
+// Every new element is read once from memory and its code written once.  Bound on prompts by the instructions per
+// value and, where K is rotated, by the fetches of its angles from the L1 cache (twice the time of the bytes); on
+// decode steps by latency: context length -> block id -> scale and rows -> codes.
 #include "cache_codes.cuh"
 #include "launch_common.cuh"
 
@@ -134,8 +135,8 @@ struct RowJob {
 };
 
 // The general way, row by row from memory: rows with infinities or NaNs (an infinity counts as the largest fp16
-// value, so that it does not take the block's scale; NaNs drop out of fmaxf), and more rows than a warp keeps
-// in registers.
+// value, so that it does not take the block's scale; NaNs drop out of fmaxf), and more rows than a warp's corner of
+// shared memory holds.
 template <bool INTERLEAVED>
 __device__ __forceinline__ void load_row_with_care(const RowJob &job, const LaneShare &l, const RotaryItem &rot, uint32_t r,
                                                    float (&x)[8], float (&y)[8]) {
@@ -232,7 +233,7 @@ constexpr uint32_t kStageBytes = PASSES * 2 * 32 * 16; // one job's rows of a wa
 // nothing but its own copies has to be waited for.  The maximum of V is taken two fp16 values at a time.  The
 // maxima propagate NaNs, so an infinity or a NaN among the inputs shows in the result.  A lane without a row of its
 // own in a group takes the last row over again: it changes no maximum and is not stored.
-// Measured on 37 376 prompt tokens (8 KV heads of 128, e4m3, rotated): rows in registers, read when their job comes,
+// Measured on 37 364 prompt tokens (8 KV heads of 128, e4m3, rotated): rows in registers, read when their job comes,
 // 79 us; with the copies ahead, pairs of values per instruction and whole runs of addresses per piece 74 us (51 us
 // without the rotation, whose angles come from the L1 cache twice for every head; 38 us is what the bytes take).
 // Layout: [row group][piece][lane], 16 bytes each.
@@ -381,7 +382,8 @@ __global__ void __launch_bounds__(kAppendThreads, 3) append_block_scaled_kernel(
   if (blockIdx.y < a.append_ctas) {
     const uint32_t heads = a.num_kv_heads;
     const LaneShare lane_share(D, lane);
-    const RotaryItem rot_k = a.rotary_dim != 0u ? rotary_item(lane_share.item, a.rotary_dim, INTERLEAVED) : plain_item(lane_share.item, D);
+    const RotaryItem rot_k = a.rotary_dim != 0u ? rotary_item(lane_share.item, a.rotary_dim, INTERLEAVED)
+                                                : plain_item(lane_share.item, D);
     const RotaryItem rot_v = plain_item(lane_share.item, D);
     const uint32_t parts = a.warps_per_job, part = warp % parts;
     const uint32_t jobs_at_once = kAppendWarps / parts;
@@ -444,8 +446,11 @@ __global__ void __launch_bounds__(kAppendThreads, 3) append_block_scaled_kernel(
         copies_wait<0>();
       }
       // two rows of the table in turn: a warp may be a round ahead of another
-      if (job.angles == nullptr) append_rows<KV, INTERLEAVED, PASSES, false>(job, lane_share, rot_v, at, part, parts, tops[round & 1u], lane, warp);
-      else append_rows<KV, INTERLEAVED, PASSES, true>(job, lane_share, rot_k, at, part, parts, tops[round & 1u], lane, warp);
+      float *const row = tops[round & 1u];
+      if (job.angles == nullptr)
+        append_rows<KV, INTERLEAVED, PASSES, false>(job, lane_share, rot_v, at, part, parts, row, lane, warp);
+      else
+        append_rows<KV, INTERLEAVED, PASSES, true>(job, lane_share, rot_k, at, part, parts, row, lane, warp);
       ++round;
     }
     return;
@@ -458,7 +463,8 @@ __global__ void __launch_bounds__(kAppendThreads, 3) append_block_scaled_kernel(
   const RotaryItem rot = rotary_item(item, a.rotary_dim, INTERLEAVED);
   const uint32_t pairs = a.tokens_per_cta * a.num_heads;
   const uint32_t step = (gridDim.y - a.append_ctas) * pairs_at_once;
-  for (uint32_t p0 = (blockIdx.y - a.append_ctas) * pairs_at_once; p0 < pairs; p0 += kQueryBatch * step) { // the same trips for all lanes: they shuffle
+  // the same trips for all lanes: they shuffle
+  for (uint32_t p0 = (blockIdx.y - a.append_ctas) * pairs_at_once; p0 < pairs; p0 += kQueryBatch * step) {
     uint4 raw[kQueryBatch][2];
     uint32_t position[kQueryBatch];
     size_t row[kQueryBatch]; // token * num_heads + head
@@ -578,7 +584,7 @@ extern "C" PA_API int pa_append_block_scaled(const pa_block_scaled_params *p, vo
   while (per_cta < 32u && per_cta * 2u <= average) per_cta *= 2u;
   a.tokens_per_cta = per_cta;
   // A few new rows per block (decode steps): one group of rows per warp, and twice the CTAs on an SM.  Otherwise four
-  // groups, and as many warps to a job as keep a block's new rows in registers.
+  // groups, and as many warps to a job as hold a block's new rows in shared memory.
   const uint32_t rows = std::min(p->block_size, average);
   const uint32_t rows_per_pass = 32u / (p->head_size / 16u);
   const bool few = rows <= rows_per_pass;
