@@ -110,8 +110,9 @@ def shard_reference_batch(case: dict, devices: Sequence, scheme: str, variant: s
     group = h // hk
     d = case["query"].size(2)
     bs = case["key_cache"].size(1)
-    fp8 = case["key_cache"].dtype != torch.float16
-    mod = getattr(lib, f"paged_attention_{'fp8_' if fp8 else ''}{variant}")
+    fp8 = case["key_cache"].dtype != torch.float16  # an 8-bit cache; `fp8_scale` is its scale
+    prefix = "int8_" if case["key_cache"].dtype == torch.int8 else "fp8_" if fp8 else ""
+    mod = getattr(lib, f"paged_attention_{prefix}{variant}")
     psize = _cabi.partition_size(d)
     plan = plan_shards(ctx, hk, len(devices), scheme)
     job = ShardedDecode(scheme)

@@ -269,3 +269,18 @@ def test_block_ids_outside_the_cache_read_zeros(cuda_device):
     case["block_tables"][0, 1] = case["key_cache"].size(0) + 7
     for variant in ("loop", "reduce"):
         check(_run(variant, case, cuda_device, **_scales(case, "block")), want, tol, variant)
+
+
+@pytest.mark.parametrize("scheme,parts", [("lpt", 3), ("heads", 2)])
+def test_shards_of_a_batch(cuda_device, scheme, parts):
+    """The multi-GPU driver on logical shards of an int8 batch: gathered, the bits of the whole batch."""
+    from flash_attention_factory_b200.multi_gpu import shard_reference_batch
+
+    case = paged_case(15, [900, 17, 2100, 640, 333], 16, 8, 128, 16, scale="scalar")
+    scale = case["k_scale"] = case["v_scale"] = max(case["k_scale"], case["v_scale"])
+    job = shard_reference_batch({**case, "fp8_scale": scale}, [cuda_device] * parts, scheme, "reduce")
+    job.run()
+    got = job.gather(torch.empty(5, 16, 128, dtype=torch.float16, device=cuda_device))
+    want, tol = attention64(case, scale, scale)
+    check(got, want, tol, scheme)
+    assert torch.equal(got.cpu(), _run("reduce", case, cuda_device, scale=scale))
