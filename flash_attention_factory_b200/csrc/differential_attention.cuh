@@ -56,7 +56,7 @@ static int enqueue_diff(const pa_params *p, cudaStream_t stream, uint32_t hpc) {
 }
 
 // KV heads per CTA (whole pairs) and tiles per stage, by the rules of ordinary attention.  (CTAs of 8 warps and 8
-// KV heads brought nothing here: 60 against 59 us on 2 x 65536 tokens of e4m3.)
+// KV heads brought nothing here: 60 against 59 us on 2 x 65536 tokens of e4m3, weights in one part.)
 template <int D, int KV>
 static int dispatch_diff_tiles(const pa_params *p, cudaStream_t stream) {
   const uint32_t hpc = p->num_kv_heads % 4u == 0u ? 4u : 2u;

@@ -572,13 +572,17 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
   // caches of ordinary attention keep them on the general path, where their order of operations was set.
   constexpr bool BLOCK_FAST = (KV == KV_I8) || (VH == 2 && KV != KV_F16);
   // Weights in two parts: the value product takes the weight rounded to fp16 and, as a second MMA on the same V
-  // fragment, the rounded rest of it, so that the rounding of the weights no longer shows.  Taken where it is
-  // the largest of the errors: differential attention over an fp16 cache, where the maps' outputs cancel (error
-  // against fp64 3.2e-4 -> 2.1e-4, that of the rounded result itself; 48 sequences up to 8192 tokens 135 -> 139 us), and
-  // the split int8 kernel, whose partial rows are rounded to fp16 as well (3.5e-4 -> 2.9e-4; 152 -> 155 us).
-  // Not for differential attention over 8-bit caches: their codes are off by 2^-8 to 2^-3, and the kernel, which
-  // converts every V code twice, would be 19 % slower (59 -> 70 us on 2 x 65536 tokens of e4m3).
-  constexpr bool TWO_PART_WEIGHTS = (VH == 2 && KV == KV_F16) || (VH == 1 && KV == KV_I8 && MODE == MODE_SPLIT);
+  // fragment, the rounded rest of it, so that the rounding of the weights (2^-11 at most, 2.1e-4 of a result on
+  // average, more where the two maps of differential attention cancel) no longer shows beside the rounding of the
+  // result, 2.1e-4 as well.  Errors against fp64 and times with one part and with two:
+  //   differential, fp16, 48 sequences up to 8192 tokens   3.2e-4 -> 2.1e-4   135 -> 138 us
+  //   differential, e4m3, 2 x 65536 tokens                 3.2e-4 -> 2.1e-4    59 ->  70 us
+  //   int8 loop, 64 x 1500 tokens, head size 64            2.8e-4 -> 2.1e-4    28 -> 29.5 us
+  //   int8 split, 128 sequences up to 8192 tokens          3.5e-4 -> 2.9e-4   152 -> 155 us (fp16 partial rows)
+  // The second case shows what it costs where the MMAs' fixed latencies are the bound (two warps to a scheduler):
+  // other orders of the MMAs, V fragments fetched ahead and weights packed later (with a third of the spills) changed
+  // nothing.  Ordinary attention over fp16 and FP8 caches takes one part.
+  constexpr bool TWO_PART_WEIGHTS = (VH == 2) || (KV == KV_I8);
   constexpr uint32_t WP = TWO_PART_WEIGHTS ? 2u : 1u; // parts of a weight
 
   const uint32_t warp = threadIdx.x >> 5;
