@@ -15,7 +15,7 @@ _LIB_NAME = "libpaged_attention_b200_test_aids.so"
 _lib = None
 
 EXPORTED_SYMBOLS = ("pa_aid_selftest_wait_timeout", "pa_aid_measure_read_bandwidth", "pa_aid_time_launches",
-                    "pa_aid_last_error")
+                    "pa_aid_diff_split", "pa_aid_last_error")
 
 
 def library_path() -> Path:
@@ -39,6 +39,9 @@ def load_library() -> ctypes.CDLL:
     lib.pa_aid_time_launches.argtypes = [ctypes.c_void_p, ctypes.POINTER(_cabi.PaParams), ctypes.c_uint32,
                                          ctypes.c_uint32, ctypes.c_void_p, ctypes.POINTER(ctypes.c_float)]
     lib.pa_aid_time_launches.restype = ctypes.c_int
+    lib.pa_aid_diff_split.argtypes = [ctypes.POINTER(_cabi.PaParams), ctypes.POINTER(ctypes.c_uint32),
+                                      ctypes.POINTER(ctypes.c_uint32)]
+    lib.pa_aid_diff_split.restype = ctypes.c_int
     lib.pa_aid_last_error.argtypes = []
     lib.pa_aid_last_error.restype = ctypes.c_char_p
     _lib = lib
@@ -66,6 +69,13 @@ def measure_read_bandwidth(ptr: int, nbytes: int, iters: int = 10, stream: int =
                                                         nbytes2, method, iters, ctypes.c_void_p(stream),
                                                         ctypes.byref(rate)))
     return float(rate.value)
+
+
+def diff_split(p: "_cabi.PaParams") -> tuple[int, int]:
+    """(tokens of a partition, rows of a copied box) of launch_kernels_diff for this argument block; needs no GPU."""
+    tokens, rows = ctypes.c_uint32(0), ctypes.c_uint32(0)
+    _check(load_library().pa_aid_diff_split(ctypes.byref(p), ctypes.byref(tokens), ctypes.byref(rows)))
+    return tokens.value, rows.value
 
 
 def time_launches(entry: str, params_list, calls: int, stream: int = 0) -> float:

@@ -166,7 +166,7 @@ struct AttnArgs {
   // context of a (sequence, head group), its normalised result goes straight to `out`, and the
   // scratch tensors are neither read nor written (they may be null)
   uint32_t whole_context_items;
-  // differential attention: the partition size in tokens, any multiple of 64, in the place of
+  // differential attention: the partition size in tokens, a multiple of 64 and of rows_per_box, in the place of
   // partition_shift; the last partition that the scratch has room for is open-ended.  0 otherwise.
   uint32_t partition_tokens;
   // max_blocks_per_seq * block_size (saturated to 32 bits): a context length beyond it is cut

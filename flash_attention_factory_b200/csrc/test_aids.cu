@@ -3,7 +3,7 @@
 // allocates device memory: a self-test of the bounded mbarrier wait and a read-only streaming
 // probe.  Both use the product's own device helpers (include/paged_attention_utils.hpp) and
 // status-word code (launch_common.cuh), compiled into this library a second time.
-#include "launch_common.cuh"
+#include "differential_attention.cuh"
 #include "paged_attention_b200_test_aids.h"
 
 namespace pa {
@@ -206,6 +206,16 @@ PA_API int pa_aid_time_launches(pa_aid_launch_fn launch, const pa_params *params
   if (rc != PA_OK) return pa::fail(rc, "time_launches: the launcher returned %d", rc);
   if (err != cudaSuccess) return pa::fail(PA_ERR_CUDA, "time_launches: %s", cudaGetErrorString(err));
   *us_per_call = ms * 1000.f / static_cast<float>(calls);
+  return PA_OK;
+}
+
+PA_API int pa_aid_diff_split(const pa_params *p, uint32_t *partition_tokens, uint32_t *box_rows) {
+  using namespace pa;
+  if (p == nullptr || partition_tokens == nullptr || box_rows == nullptr)
+    return fail(PA_ERR_BAD_ARG, "diff_split: null argument");
+  if (int rc = validate_params(p, p->kv_dtype != PA_KV_F16, /*needs_scratch=*/true, p->kv_dtype == PA_KV_INT8)) return rc;
+  *partition_tokens = diff_partition_tokens(p);
+  *box_rows = diff_box_rows(p);
   return PA_OK;
 }
 

@@ -199,8 +199,9 @@ PA_API int launch_kernels_int8_reduce(const pa_params *p, void *stream, float *u
  *   kv_dtype       any pa_kv_dtype; scales as in the FP8 and int8 entry points, per cache head
  *   sinks, alibi_slopes, softcap  must be off
  * A context is cut into at most max_num_partitions partitions of P tokens, P = max_context_len /
- * max_num_partitions rounded up to a multiple of 64; the last one is open-ended, so a result never
- * misses a token whatever max_context_len says. */
+ * max_num_partitions rounded up to a multiple of 64 (of 128 for an 8-bit cache of head size 64 and
+ * blocks of 128 with an odd number of pairs, whose copies are 128 rows high); the last one is
+ * open-ended, so a result never misses a token whatever max_context_len says. */
 typedef struct pa_diff_params {
   pa_params attn;
   const float *lambdas;     /* fp32 [H]: the learned weight of the second map */

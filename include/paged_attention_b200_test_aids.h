@@ -48,6 +48,10 @@ typedef int (*pa_aid_launch_fn)(const pa_params *p, void *stream, float *us_out)
 PA_API int pa_aid_time_launches(pa_aid_launch_fn launch, const pa_params *params, uint32_t num_params,
                                 uint32_t calls, void *stream, float *us_per_call);
 
+/* How launch_kernels_diff cuts the contexts of an argument block: the tokens of a partition and the rows
+ * of a cache block that one copy takes.  Host arithmetic only. */
+PA_API int pa_aid_diff_split(const pa_params *p, uint32_t *partition_tokens, uint32_t *box_rows);
+
 /* Message of the last non-PA_OK return of this library on the calling thread. */
 PA_API const char *pa_aid_last_error(void);
 
