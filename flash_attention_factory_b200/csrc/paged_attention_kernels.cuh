@@ -194,6 +194,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 // steps larger than this (log2 units), so weights stay below 2^8 and most tiles skip
 // the rescaling of the accumulator.
 constexpr float kRescaleThreshold = 8.0f;
+// The softmax scale of keys whose dequantisation scale is 0 (they are zeros): every score within fp16's and the
+// codes' range times this is 0 beside the reference, and -inf times it stays -inf where 0 would make a NaN.
+constexpr float kZeroScale = 1e-30f;
 
 template <int D, int KV, int NWARPS = 4, int TILES = 1, int VH = 1>
 struct SmemLayout {
@@ -1098,7 +1101,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
     const uint32_t box_shift = 31u - __clz(args.rows_per_box); // a power of two, like both it is the smaller of
     auto tile_scales = [&](uint32_t stage_slot, uint32_t row, float &k_scale, float (&v)[VH]) {
       const float2 *s = stage_scales + stage_slot * L::SCALE_SLOTS + (row >> box_shift) * hpc;
-      k_scale = fmaxf(args.sm_scale_log2 * kKeyUnit * s[my_head].x, 1e-30f);
+      k_scale = fmaxf(args.sm_scale_log2 * kKeyUnit * s[my_head].x, kZeroScale);
 #pragma unroll
       for (uint32_t vh = 0; vh < VH; ++vh) v[vh] = s[v_head0 + vh].y;
     };
@@ -1109,10 +1112,11 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
       nxt.valid = false;
       const uint32_t kv_head = cur.head_base + my_head;
       // softmax scale (log2 domain) and output scale of this warp's KV head
-      const float scale = ((args.k_scale_per_head != nullptr)
-                               ? args.sm_scale_log2 * __ldg(args.k_scale_per_head + kv_head)
-                               : args.scale_log2) *
-                          kKeyUnit;
+      float scale = ((args.k_scale_per_head != nullptr) ? args.sm_scale_log2 * __ldg(args.k_scale_per_head + kv_head)
+                                                        : args.scale_log2) *
+                    kKeyUnit;
+      // a head of zeros: as in tile_scales, a tiny positive scale weighs all tokens alike and keeps a masked -inf
+      if (KV != KV_F16 && scale == 0.f) scale = kZeroScale;
       float out_scale[VH];
 #pragma unroll
       for (uint32_t vh = 0; vh < VH; ++vh)

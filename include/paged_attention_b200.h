@@ -96,7 +96,8 @@ typedef struct pa_params {
    * [num_kv_heads] each, or NULL).  The reference has one scalar fp8_scale
    * (paged_attention_fp8_loop/paged_attention_fp8_loop.cpp:34); when these are set,
    * K of head k dequantises as fp16(code) * k_scale_per_head[k] and V as
-   * fp16(code) * v_scale_per_head[k], and fp8_scale is not used for that cache. */
+   * fp16(code) * v_scale_per_head[k], and fp8_scale is not used for that cache.  A scale of 0 is
+   * a head of zeros. */
   const float *k_scale_per_head;
   const float *v_scale_per_head;
   /* Opt-in score modifiers.  The reference accepts alibi_slopes and softcap and ignores
