@@ -571,8 +571,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
   float2 *stage_scales = reinterpret_cast<float2 *>(smem + L::SCALES_OFFSET); // [NSTAGES][SCALE_SLOTS]
   const bool block_scales = (KV != KV_F16) && args.k_scale_per_block != nullptr;
   // Per-block scales of an int8 cache, and of any cache in differential attention, are folded into the
-  // straight-line path too, with a running reference for the V scales (see fold_v_scales); the FP8
-  // caches of ordinary attention keep them on the general path, where their order of operations was set.
+  // straight-line path too; the FP8 caches of ordinary attention keep them on the general path, so that their
+  // straight-line path, without block scales, stays as it is.  Both keep a running reference for the V scales (see
+  // fold_v_scales).
   constexpr bool BLOCK_FAST = (KV == KV_I8) || (VH == 2 && KV != KV_F16);
   // Weights in two parts: the value product takes the weight rounded to fp16 and, as a second MMA on the same V
   // fragment, the rounded rest of it, so that the rounding of the weights (2^-11 at most, 2.1e-4 of a result on
@@ -1045,10 +1046,11 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
         }
       }
     };
-    // Running reference of the V block scales (BLOCK_FAST): a tile's weights are multiplied by its
+    // Running reference of the V block scales: a tile's weights are multiplied by its
     // scale over the largest scale so far, a factor of at most 1, before they are rounded to fp16,
     // and the accumulator carries the reference; multiplying by the scale itself would push the
-    // weights of a cache with small values into the subnormal halves.  Uniform across the warp;
+    // weights of a cache with small values into the subnormal halves (a block scale of e5m2 is its largest value
+    // over 57344: 1.7e-5 for values of 1, below every normal half already).  Uniform across the warp;
     // the reference grows about ln(blocks) times per item.
     float v_ref = 0.f, v_inv = 0.f;
     auto fold_v_scales = [&](const float (&va)[VH], const float (&vb)[VH], float (&wa)[VH], float (&wb)[VH]) {
@@ -1286,10 +1288,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
             cb[0] = cb[1] = cb[2] = cb[3] = neg_infinity();
           }
           float eff_scale = scale;
-          float v_scale_a = 1.f, v_scale_b = 1.f; // per-block V scales of the two tiles
           float k_nat_a = scale * kLn2, k_nat_b = scale * kLn2; // sm_scale * k scale of the two tiles
-          float s_a = scale, s_b = scale; // BLOCK_FAST: softmax scales of the two tiles,
-          float w_a[VH], w_b[VH];         // and their V scales over the reference
+          float s_a = scale, s_b = scale; // BLOCK_FAST: softmax scales of the two tiles
+          float w_a[VH], w_b[VH];         // per-block scales: V scales of the two tiles over the reference
           if constexpr (BLOCK_FAST) {
             if (block_scales) {
               float v_a[VH], v_b[VH];
@@ -1304,14 +1305,14 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
             }
           } else if (block_scales) {
             // tile A / B lie in one KV block each: the stage's slot for (that block, this head)
-            const uint32_t chunk_a = (sub_a * tpt + my_slice * 16u) / args.rows_per_box;
-            const uint32_t chunk_b = (sub_b * tpt + my_slice * 16u) / args.rows_per_box;
+            const uint32_t chunk_a = (sub_a * tpt + my_slice * 16u) >> box_shift;
+            const uint32_t chunk_b = (sub_b * tpt + my_slice * 16u) >> box_shift;
             const float2 sa = stage_scales[slot_a * L::SCALE_SLOTS + chunk_a * hpc + my_head];
             const float2 sb2 = act_b ? stage_scales[slot_b * L::SCALE_SLOTS + chunk_b * hpc + my_head] : make_float2(1.f, 1.f);
             k_nat_a = args.sm_scale_log2 * kLn2 * sa.x;
             k_nat_b = args.sm_scale_log2 * kLn2 * sb2.x;
-            v_scale_a = sa.y;
-            v_scale_b = sb2.y;
+            const float v_a[VH] = {sa.y}, v_b[VH] = {act_b ? sb2.y : 0.f};
+            fold_v_scales(v_a, v_b, w_a, w_b);
           }
           if (modifiers) {
             // soft-cap / ALiBi / per-block scales: turn the raw dot products into log2-domain
@@ -1373,11 +1374,11 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
           l_run[1] += (pa[1] + pa[3]) + (pb[1] + pb[3]);
           const bool weighted = BLOCK_FAST && block_scales;
           if (block_scales && !BLOCK_FAST) {
-            // V of a block dequantises as code * scale: fold the scale into the weights
+            // V of a block dequantises as code * scale: fold the scale, over the reference, into the weights
 #pragma unroll
             for (uint32_t j = 0; j < 4; ++j) {
-              pa[j] *= v_scale_a;
-              pb[j] *= v_scale_b;
+              pa[j] *= w_a[0];
+              pb[j] *= w_b[0];
             }
           }
           // P rounded to fp16 for the MMA, transposed into the B-operand layout;
@@ -1437,7 +1438,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
       l_run[1] = quad_column_sum(l_run[1]);
       const bool ok = (*abort_flag == 0u);
       // with folded V scales the accumulator is relative to this warp's reference scale
-      const float acc_scale = (BLOCK_FAST && block_scales) ? v_ref : 1.f;
+      const float acc_scale = block_scales ? v_ref : 1.f;
 
       if constexpr (MODE == MODE_SPLIT) {
         if (hpc == NW) {
