@@ -330,28 +330,29 @@ __device__ __forceinline__ void fetch_rows(const RowJob &job, const LaneShare &l
   copies_commit();
 }
 
-// K (ROTATE) or V rows of one (block, head) by `parts` warps, of which this is number `part`.
-template <int KV, bool INTERLEAVED, int PASSES, bool ROTATE>
-__device__ __forceinline__ void append_rows(const RowJob &job, const LaneShare &l, const RotaryItem &rot, uint32_t at,
-                                            uint32_t part, uint32_t parts, float *tops, uint32_t lane, uint32_t warp) {
-  const HeldRows<PASSES, ROTATE, INTERLEAVED> rows{job, l, rot, at};
-  bool careful = true;
+// Largest magnitude among a job's rows of this warp, in all lanes; `careful` if infinities or NaNs or their number call
+// for the general way.
+template <bool INTERLEAVED, int PASSES, bool ROTATE>
+__device__ __forceinline__ float largest_of_rows(const RowJob &job, const LaneShare &l, const RotaryItem &rot, uint32_t at,
+                                                 bool &careful) {
+  careful = true;
   float top = 0.f;
   if (job.in_stage) {
-    top = rows.largest();
+    top = HeldRows<PASSES, ROTATE, INTERLEAVED>{job, l, rot, at}.largest();
     careful = __any_sync(0xffffffffu, !(top <= 1e30f)) != 0;
   }
   if (careful && job.live) top = largest_with_care<INTERLEAVED>(job, l, rot);
-  top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))); // magnitudes order like their bits
-  if (parts > 1u) { // the largest value of the job's warps
-    if (lane == 0) tops[warp] = top;
-    __syncthreads();
-    for (uint32_t k = 0; k < parts; ++k) top = fmaxf(top, tops[warp - part + k]);
-  }
-  if (!job.live) return;
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))); // magnitudes order like their bits
+}
+
+// The rest of a live job, once `top`, the largest magnitude among the rows of all its `parts` warps, is known: new
+// codes by this one, number `part`, and its share of the held rows.
+template <int KV, bool INTERLEAVED, int PASSES, bool ROTATE>
+__device__ __forceinline__ void store_rows(const RowJob &job, const LaneShare &l, const RotaryItem &rot, uint32_t at,
+                                           bool careful, float top, uint32_t part, uint32_t parts, uint32_t lane) {
   const float grown = fmaxf(job.held, __fdiv_rn(top, largest_code<KV>()));
   const float scale = (grown > 0.f) ? grown : 1.f; // a block of zeros keeps scale 0 and codes 0
-  if (!careful && !Divider(scale).plain) rows.template store<KV>(scale);
+  if (!careful && !Divider(scale).plain) HeldRows<PASSES, ROTATE, INTERLEAVED>{job, l, rot, at}.template store<KV>(scale);
   else store_with_care<KV, INTERLEAVED>(job, l, rot, scale);
   if (grown > job.held && l.active) {
     const uint32_t r = part * l.rows_per_pass + l.row, step = parts * l.rows_per_pass;
@@ -360,7 +361,7 @@ __device__ __forceinline__ void append_rows(const RowJob &job, const LaneShare &
                           divide_round_up(job.first_row - r, step), job.held, scale);
   }
   // every lane of the job's warps has read the old scale: this warp's before its copies were waited for, the others'
-  // before the barrier above
+  // before the barrier between the two functions
   if (lane == 0 && part == 0u) *job.scale_at = grown;
 }
 
@@ -445,12 +446,23 @@ __global__ void __launch_bounds__(kAppendThreads, 3) append_block_scaled_kernel(
       } else {
         copies_wait<0>();
       }
-      // two rows of the table in turn: a warp may be a round ahead of another
-      float *const row = tops[round & 1u];
-      if (job.angles == nullptr)
-        append_rows<KV, INTERLEAVED, PASSES, false>(job, lane_share, rot_v, at, part, parts, row, lane, warp);
-      else
-        append_rows<KV, INTERLEAVED, PASSES, true>(job, lane_share, rot_k, at, part, parts, row, lane, warp);
+      const bool rotated = job.angles != nullptr;
+      bool careful;
+      float top = rotated ? largest_of_rows<INTERLEAVED, PASSES, true>(job, lane_share, rot_k, at, careful)
+                          : largest_of_rows<INTERLEAVED, PASSES, false>(job, lane_share, rot_v, at, careful);
+      if (parts > 1u) {
+        // The largest value of the job's warps.  Warps with K and with V jobs, or with none, meet at this one barrier: all
+        // warps of the CTA make the same number of rounds.  Two rows of the table in turn: a warp may be a round ahead
+        // of another.
+        float *const row = tops[round & 1u];
+        if (lane == 0) row[warp] = top;
+        __syncthreads();
+        for (uint32_t k = 0; k < parts; ++k) top = fmaxf(top, row[warp - part + k]);
+      }
+      if (job.live) {
+        if (rotated) store_rows<KV, INTERLEAVED, PASSES, true>(job, lane_share, rot_k, at, careful, top, part, parts, lane);
+        else store_rows<KV, INTERLEAVED, PASSES, false>(job, lane_share, rot_v, at, careful, top, part, parts, lane);
+      }
       ++round;
     }
     return;
