@@ -130,8 +130,15 @@ def enqueue(max_logits, exp_sums, tem_output, output, query, key_cache, value_ca
     _launch.call(_cabi.load_library().launch_kernels_diff, q, query.get_device(), None)
 
 
-def run(*args, **kwargs) -> list[float]:
+def run(max_logits, exp_sums, tem_output, output, query, key_cache, value_cache, block_tables, context_lens,
+        lambdas, sm_scale, kv_scale, block_size, max_context_len, *, norm_weight=None, norm_eps=1e-5,
+        norm_scale=1.0, k_scale_per_head=None, v_scale_per_head=None, k_scale_per_block=None,
+        v_scale_per_block=None) -> list[float]:
     """``enqueue``, blocking; returns device microseconds [attention, merge]."""
+    q = params(max_logits, exp_sums, tem_output, output, query, key_cache, value_cache, block_tables, context_lens,
+               lambdas, sm_scale, kv_scale, block_size, max_context_len, norm_weight=norm_weight, norm_eps=norm_eps,
+               norm_scale=norm_scale, k_scale_per_head=k_scale_per_head, v_scale_per_head=v_scale_per_head,
+               k_scale_per_block=k_scale_per_block, v_scale_per_block=v_scale_per_block)
     us = (ctypes.c_float * 2)()
-    _launch.call(_cabi.load_library().launch_kernels_diff, params(*args, **kwargs), args[4].get_device(), us)
+    _launch.call(_cabi.load_library().launch_kernels_diff, q, query.get_device(), us)
     return [float(us[0]), float(us[1])]
