@@ -235,7 +235,9 @@ extern "C" PA_API uint32_t pa_diff_num_partitions(uint32_t num_seqs, uint32_t nu
   // 127 us with 256 tokens, 138 with 512, 167 with 1024, 149 with 171).
   const uint32_t hpc = num_kv_heads % 4u == 0u ? 4u : 2u;
   const uint32_t token_bytes = hpc * head_size * 2u * (kv_dtype == PA_KV_F16 ? 2u : 1u);
-  const uint32_t usual = divide_round_up(max_context_len, (512u << 10) / token_bytes);
+  const uint64_t longest = max_context_len; // 64 bits: rounding a hint of nearly 2^32 up passes 32
+  const uint32_t usual_tokens = (512u << 10) / token_bytes;
+  const uint64_t usual = (longest + usual_tokens - 1u) / usual_tokens;
   const uint64_t units = static_cast<uint64_t>(num_seqs) * (num_kv_heads / hpc);
   const uint64_t items = units * usual, slots = 296u; // CTAs resident on 148 SMs
   uint64_t parts = usual;
@@ -245,7 +247,7 @@ extern "C" PA_API uint32_t pa_diff_num_partitions(uint32_t num_seqs, uint32_t nu
   if (items < 4u * slots) {
     const uint64_t rounds = std::max<uint64_t>(1u, items / slots);
     parts = std::max<uint64_t>(1u, rounds * slots / units);
-    parts = std::min<uint64_t>(parts, divide_round_up(max_context_len, 64u));
+    parts = std::min<uint64_t>(parts, (longest + 63u) / 64u);
   }
   return static_cast<uint32_t>(std::min<uint64_t>(65535u, parts)); // the kernel's index arithmetic
 }

@@ -34,7 +34,8 @@ def scratch(query: torch.Tensor, key_cache: torch.Tensor, max_context_len: int):
     [S, 2 H, NP, 2 D].  NP sets how finely a context is split; any NP >= 1 gives a correct result."""
     s, h2, d = query.shape
     kv_dtype = _kv_dtype(key_cache)
-    npart = int(_cabi.load_library().pa_diff_num_partitions(s, key_cache.size(2), d, max(0, int(max_context_len)), kv_dtype))
+    hint = max(0, min(int(max_context_len), 0xFFFFFFFF))
+    npart = int(_cabi.load_library().pa_diff_num_partitions(s, key_cache.size(2), d, hint, kv_dtype))
     _shim._require(npart > 0, "Unsupported head size or number of KV heads")
     stats = torch.empty(2, s, h2, npart, dtype=torch.float32, device=query.device)
     return stats[0], stats[1], torch.empty(s, h2, npart, 2 * d, dtype=torch.float32, device=query.device)

@@ -30,3 +30,22 @@ def test_blocking_differential_attention_with_keywords(cuda_device):
                 v_scale_per_block=c["v_scale"])
         assert fn is diff.enqueue or len(us) == 2
     assert torch.equal(*outs)
+
+
+def test_partition_counts_of_the_largest_hints():
+    """A hint near 2^32 is a long context, not an overflow; one beyond it is the largest."""
+    import torch
+
+    from flash_attention_factory_b200 import _cabi, build
+    from flash_attention_factory_b200.lib import paged_attention_diff as diff
+
+    build.build()
+    n = _cabi.load_library().pa_diff_num_partitions
+    for kv in range(4):
+        for heads in (2, 8):
+            for seqs in (1, 3, 3000):
+                counts = [n(seqs, heads, 64, hint, kv) for hint in (2 ** 31, 2 ** 32 - 2000, 2 ** 32 - 64, 2 ** 32 - 1)]
+                assert counts == [counts[0]] * 4 and counts[0] >= 1, (kv, heads, seqs, counts)
+    cache = torch.empty(1, 16, 2, 64, dtype=torch.float16)
+    scratch = diff.scratch(torch.empty(1, 2, 64, dtype=torch.float16, device="meta"), cache, 2 ** 40)
+    assert scratch[0].shape[2] == n(1, 2, 64, 2 ** 32 - 1, 0)
