@@ -71,13 +71,13 @@ class AutoDecodePlan:
 def paged_attention_auto(plan: AutoDecodePlan, out, query, key_cache, value_cache, block_tables,
                          context_lens, num_queries_per_tokens: int, sm_scale: float,
                          fp8_scale: float = 1.0, sinks=None, *, k_scale_per_block=None,
-                         v_scale_per_block=None) -> None:
+                         v_scale_per_block=None, k_scale_per_head=None, v_scale_per_head=None) -> None:
     """Asynchronous decode attention of a whole batch: loop kernel for the plan's short
     sequences, split-context pair for its long ones.  Both launches work on the caller's
     tensors in place (each is given the list of sequence ids it covers), on two streams that
     fork from and join the current stream.  `out` [S, H, D] is written for every sequence.
-    The entry points follow the cache's type (fp16, FP8, int8); `fp8_scale` or the per-block scales
-    are those of an 8-bit cache."""
+    The entry points follow the cache's type (fp16, FP8, int8); `fp8_scale`, the per-block or the
+    per-head scales are those of an 8-bit cache."""
     fp8 = key_cache.dtype != torch.float16  # an 8-bit cache
     int8 = key_cache.dtype == torch.int8
     prefix = "int8_" if int8 else "fp8_" if fp8 else ""
@@ -87,7 +87,8 @@ def paged_attention_auto(plan: AutoDecodePlan, out, query, key_cache, value_cach
         p = _shim.build_params(plan.max_logits, plan.exp_sums, plan.tmp_out, out, None, query, key_cache,
                                value_cache, block_tables, context_lens, num_queries_per_tokens, sm_scale,
                                fp8_scale, key_cache.size(1), sub.max_ctx, plan.alibi, sinks, -1.0, fp8=fp8,
-                               int8=int8, k_scale_per_block=k_scale_per_block, v_scale_per_block=v_scale_per_block)
+                               int8=int8, k_scale_per_block=k_scale_per_block, v_scale_per_block=v_scale_per_block,
+                               k_scale_per_head=k_scale_per_head, v_scale_per_head=v_scale_per_head)
         if variant == "reduce":
             _shim.check_scratch(p, plan.max_logits, plan.exp_sums, plan.tmp_out)
         if sub.count != query.size(0):

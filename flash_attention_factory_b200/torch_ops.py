@@ -46,10 +46,14 @@ def fp8_loop(max_logits: torch.Tensor, exp_sums: torch.Tensor, tem_output: torch
              query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, block_tables: torch.Tensor,
              context_lens: torch.Tensor, num_queries_per_tokens: int, sm_scale: float, fp8_scale: float,
              block_size: int, max_context_len: int, alibi_slopes: torch.Tensor, sinks: Optional[torch.Tensor],
-             softcap: float) -> None:
+             softcap: float, k_scale_per_block: Optional[torch.Tensor] = None,
+             v_scale_per_block: Optional[torch.Tensor] = None, k_scale_per_head: Optional[torch.Tensor] = None,
+             v_scale_per_head: Optional[torch.Tensor] = None) -> None:
     paged_attention_fp8_loop.enqueue(max_logits, exp_sums, tem_output, output, None, query, key_cache,
                                      value_cache, block_tables, context_lens, num_queries_per_tokens, sm_scale,
-                                     fp8_scale, block_size, max_context_len, alibi_slopes, sinks, softcap)
+                                     fp8_scale, block_size, max_context_len, alibi_slopes, sinks, softcap,
+                                     k_scale_per_block=k_scale_per_block, v_scale_per_block=v_scale_per_block,
+                                     k_scale_per_head=k_scale_per_head, v_scale_per_head=v_scale_per_head)
 
 
 @torch.library.custom_op("paged_attention_b200::fp8_reduce", mutates_args=_MUTATED)
@@ -57,10 +61,14 @@ def fp8_reduce(max_logits: torch.Tensor, exp_sums: torch.Tensor, tem_output: tor
                query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, block_tables: torch.Tensor,
                context_lens: torch.Tensor, num_queries_per_tokens: int, sm_scale: float, fp8_scale: float,
                block_size: int, max_context_len: int, alibi_slopes: torch.Tensor, sinks: Optional[torch.Tensor],
-               softcap: float) -> None:
+               softcap: float, k_scale_per_block: Optional[torch.Tensor] = None,
+               v_scale_per_block: Optional[torch.Tensor] = None, k_scale_per_head: Optional[torch.Tensor] = None,
+               v_scale_per_head: Optional[torch.Tensor] = None) -> None:
     paged_attention_fp8_reduce.enqueue(max_logits, exp_sums, tem_output, output, None, query, key_cache,
                                        value_cache, block_tables, context_lens, num_queries_per_tokens, sm_scale,
-                                       fp8_scale, block_size, max_context_len, alibi_slopes, sinks, softcap)
+                                       fp8_scale, block_size, max_context_len, alibi_slopes, sinks, softcap,
+                                       k_scale_per_block=k_scale_per_block, v_scale_per_block=v_scale_per_block,
+                                       k_scale_per_head=k_scale_per_head, v_scale_per_head=v_scale_per_head)
 
 
 @torch.library.custom_op("paged_attention_b200::int8_loop", mutates_args=_MUTATED)
@@ -69,11 +77,13 @@ def int8_loop(max_logits: torch.Tensor, exp_sums: torch.Tensor, tem_output: torc
               context_lens: torch.Tensor, num_queries_per_tokens: int, sm_scale: float, int8_scale: float,
               block_size: int, max_context_len: int, alibi_slopes: torch.Tensor, sinks: Optional[torch.Tensor],
               softcap: float, k_scale_per_block: Optional[torch.Tensor] = None,
-              v_scale_per_block: Optional[torch.Tensor] = None) -> None:
+              v_scale_per_block: Optional[torch.Tensor] = None, k_scale_per_head: Optional[torch.Tensor] = None,
+              v_scale_per_head: Optional[torch.Tensor] = None) -> None:
     paged_attention_int8_loop.enqueue(max_logits, exp_sums, tem_output, output, None, query, key_cache,
                                       value_cache, block_tables, context_lens, num_queries_per_tokens, sm_scale,
                                       int8_scale, block_size, max_context_len, alibi_slopes, sinks, softcap,
-                                      k_scale_per_block=k_scale_per_block, v_scale_per_block=v_scale_per_block)
+                                      k_scale_per_block=k_scale_per_block, v_scale_per_block=v_scale_per_block,
+                                      k_scale_per_head=k_scale_per_head, v_scale_per_head=v_scale_per_head)
 
 
 @torch.library.custom_op("paged_attention_b200::int8_reduce", mutates_args=_MUTATED)
@@ -82,11 +92,13 @@ def int8_reduce(max_logits: torch.Tensor, exp_sums: torch.Tensor, tem_output: to
               context_lens: torch.Tensor, num_queries_per_tokens: int, sm_scale: float, int8_scale: float,
               block_size: int, max_context_len: int, alibi_slopes: torch.Tensor, sinks: Optional[torch.Tensor],
               softcap: float, k_scale_per_block: Optional[torch.Tensor] = None,
-              v_scale_per_block: Optional[torch.Tensor] = None) -> None:
+              v_scale_per_block: Optional[torch.Tensor] = None, k_scale_per_head: Optional[torch.Tensor] = None,
+              v_scale_per_head: Optional[torch.Tensor] = None) -> None:
     paged_attention_int8_reduce.enqueue(max_logits, exp_sums, tem_output, output, None, query, key_cache,
                                       value_cache, block_tables, context_lens, num_queries_per_tokens, sm_scale,
                                       int8_scale, block_size, max_context_len, alibi_slopes, sinks, softcap,
-                                      k_scale_per_block=k_scale_per_block, v_scale_per_block=v_scale_per_block)
+                                      k_scale_per_block=k_scale_per_block, v_scale_per_block=v_scale_per_block,
+                                      k_scale_per_head=k_scale_per_head, v_scale_per_head=v_scale_per_head)
 
 
 @torch.library.custom_op("paged_attention_b200::diff", mutates_args=_MUTATED)
@@ -105,8 +117,8 @@ def diff(max_logits: torch.Tensor, exp_sums: torch.Tensor, tem_output: torch.Ten
 
 
 @torch.library.custom_op("paged_attention_b200::rope_and_cache", mutates_args=("query_out", "key_cache", "value_cache"))
-def rope_and_cache(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, positions: torch.Tensor,
-                   cos_sin: torch.Tensor, query_out: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+def rope_and_cache(query: Optional[torch.Tensor], key: torch.Tensor, value: torch.Tensor, positions: torch.Tensor,
+                   cos_sin: torch.Tensor, query_out: Optional[torch.Tensor], key_cache: torch.Tensor, value_cache: torch.Tensor,
                    slot_mapping: torch.Tensor, fp8_scale: float = 1.0, interleaved: bool = False,
                    k_scale_per_head: Optional[torch.Tensor] = None, v_scale_per_head: Optional[torch.Tensor] = None,
                    k_scale_per_block: Optional[torch.Tensor] = None,
