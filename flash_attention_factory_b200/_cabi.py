@@ -81,7 +81,7 @@ class PaParams(ctypes.Structure):
         ("sm_scale", ctypes.c_float),
         ("fp8_scale", ctypes.c_float),
         ("kv_dtype", ctypes.c_int32),
-        ("reserved1", ctypes.c_int32),
+        ("tmp_out_f32", ctypes.c_int32),
         ("k_scale_per_head", ctypes.c_void_p),
         ("v_scale_per_head", ctypes.c_void_p),
         ("alibi_slopes", ctypes.c_void_p),

@@ -266,7 +266,8 @@ PA_API int pa_decode_step_host_batch(int32_t entry, const pa_params *p, const pa
       const size_t stat_rows = static_cast<size_t>(lo) * p->num_heads * p->max_num_partitions;
       sub.max_logits = advance(p->max_logits, stat_rows * sizeof(float));
       sub.exp_sums = advance(p->exp_sums, stat_rows * sizeof(float));
-      sub.tmp_out = advance(p->tmp_out, stat_rows * p->head_size * 2);
+      const size_t partial_bytes = (entry == PA_ENTRY_INT8_REDUCE && p->tmp_out_f32 != 0) ? 4u : 2u;
+      sub.tmp_out = advance(p->tmp_out, stat_rows * p->head_size * partial_bytes);
     }
     const bool direct = direct_last && k + 1 == n;
     if (direct) sub.out = advance(io->host_out, lo * row_bytes); // the kernels write the host buffer themselves

@@ -351,6 +351,7 @@ AttnArgs make_attn_args(const pa_params *p, uint32_t hpc) {
   a.ctx_limit = context_limit(p);
   a.partition_shift = log2_pow2(policy::partition_size);
   a.whole_context_items = 0u;
+  a.partials_f32 = (KV == KV_I8 && p->tmp_out_f32 != 0) ? 1u : 0u;
   a.table_offsets = p->block_table_offsets;
   a.hpc = hpc;
   a.tokens_per_stage = policy::tokens_per_stage / a.hpc;
@@ -458,7 +459,8 @@ static int enqueue_attention(const pa_params *p, cudaStream_t stream, uint32_t h
   return PA_OK;
 }
 
-template <int D>
+// T: type of the partial rows
+template <int D, typename T>
 static int enqueue_merge(const pa_params *p, cudaStream_t stream) {
   const uint32_t psize = (D == 64) ? 256u : 512u;
   cudaLaunchConfig_t cfg{};
@@ -490,16 +492,16 @@ static int enqueue_merge(const pa_params *p, cudaStream_t stream) {
   const bool many_pairs = pairs >= (parts > 32u ? 4096u : 2048u);
   if (forced == 2 || (forced == 0 && many_pairs)) {
     cfg.gridDim = dim3(static_cast<unsigned>((pairs + 3) / 4), 1, 1);
-    PA_CUDA_TRY(cudaLaunchKernelEx(&cfg, merge_partitions_warp_kernel<D>, static_cast<__half *>(p->out),
-                                   static_cast<const __half *>(p->tmp_out),
+    PA_CUDA_TRY(cudaLaunchKernelEx(&cfg, merge_partitions_warp_kernel<D, T>, static_cast<__half *>(p->out),
+                                   static_cast<const T *>(p->tmp_out),
                                    static_cast<const float *>(p->max_logits),
                                    static_cast<const float *>(p->exp_sums), p->context_lens, p->seq_indices,
                                    p->num_heads, static_cast<uint32_t>(pairs), p->max_num_partitions, psize,
                                    context_limit(p), p->block_table_offsets, log2_pow2(p->block_size)));
     return PA_OK;
   }
-  PA_CUDA_TRY(cudaLaunchKernelEx(&cfg, merge_partitions_kernel<D>, static_cast<__half *>(p->out),
-                                 static_cast<const __half *>(p->tmp_out),
+  PA_CUDA_TRY(cudaLaunchKernelEx(&cfg, merge_partitions_kernel<D, T>, static_cast<__half *>(p->out),
+                                 static_cast<const T *>(p->tmp_out),
                                  static_cast<const float *>(p->max_logits),
                                  static_cast<const float *>(p->exp_sums), p->context_lens, p->seq_indices,
                                  p->num_heads, p->max_num_partitions, psize, context_limit(p),
@@ -638,9 +640,10 @@ static int dispatch_head_size(const pa_params *p, cudaStream_t stream) {
   return dispatch_stage_tiles<64, KV, MODE>(p, stream);
 }
 
-static inline int dispatch_merge(const pa_params *p, cudaStream_t stream) {
-  if (p->head_size == 128) return enqueue_merge<128>(p, stream);
-  return enqueue_merge<64>(p, stream);
+template <typename T = __half>
+static int dispatch_merge(const pa_params *p, cudaStream_t stream) {
+  if (p->head_size == 128) return enqueue_merge<128, T>(p, stream);
+  return enqueue_merge<64, T>(p, stream);
 }
 
 // A -DPA_TIMELINE build exports, per launcher, a reader of its unit's time-stamp table

@@ -169,6 +169,8 @@ struct AttnArgs {
   // differential attention: the partition size in tokens, a multiple of 64 and of rows_per_box, in the place of
   // partition_shift; the last partition that the scratch has room for is open-ended.  0 otherwise.
   uint32_t partition_tokens;
+  // split mode over an int8 cache: tmp_out holds fp32 partial rows
+  uint32_t partials_f32;
   // max_blocks_per_seq * block_size (saturated to 32 bits): a context length beyond it is cut
   // to it, so no block-table read leaves the sequence's row whatever context_lens holds
   uint32_t ctx_limit;
@@ -1460,7 +1462,16 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
               if constexpr (VH == 1) {
                 const float inv = (l_run[j] > 0.f) ? (out_scale[0] * acc_scale / l_run[j]) : 0.f;
                 __half *dst = whole ? args.out + head * D : args.tmp_out + pidx * D;
-                if constexpr (KV == KV_F16) {
+                if (KV == KV_I8 && args.partials_f32 != 0u && !whole) {
+                  float *row = reinterpret_cast<float *>(args.tmp_out) + pidx * D;
+#pragma unroll
+                  for (uint32_t q = 0; q < KSTEPS / 2; ++q) {
+                    *reinterpret_cast<float2 *>(row + q * 32 + 2 * gid) =
+                        make_float2(acc[0][2 * q][j] * inv, acc[0][2 * q + 1][j] * inv);
+                    *reinterpret_cast<float2 *>(row + q * 32 + 16 + 2 * gid) =
+                        make_float2(acc[0][2 * q][2 + j] * inv, acc[0][2 * q + 1][2 + j] * inv);
+                  }
+                } else if constexpr (KV == KV_F16) {
 #pragma unroll
                   for (uint32_t i = 0; i < KSTEPS; ++i) {
                     dst[i * 16 + gid] = __float2half_rn(acc[0][i][j] * inv);
@@ -1589,7 +1600,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
                     (args.v_scale_per_head != nullptr) ? __ldg(args.v_scale_per_head + v_head) : args.out_scale;
                 const float inv = (l_all > 0.f) ? (head_scale / l_all) : 0.f;
                 const bool whole = args.whole_context_items != 0u;
-                if constexpr (VH == 1) {
+                if (VH == 1 && (KV != KV_I8 || args.partials_f32 == 0u || whole)) {
                   uint4 packed;
                   packed.x = pack_half2(lo.x * inv, lo.y * inv);
                   packed.y = pack_half2(lo.z * inv, lo.w * inv);
@@ -1699,28 +1710,67 @@ __device__ __forceinline__ uint32_t merge_context(const uint32_t *context_lens, 
 //   out[d] = sum_p (w_p / W) * tmp_out[p, d]
 // over the partitions p < ceil(ctx / partition_size) only
 // (reference paged_attention_kernel_v2.hpp:679,736-764,813-863,924-932).
-// Latency-bound: a thread owns 4 dims (one 8-byte load) of kMergeUnroll partial rows, which
+// Latency-bound: a thread owns 4 dims (one 8-byte load) of UNROLL partial rows, which
 // are requested together with the statistics, before the weights are known; up to
-// kMergeUnroll * ROWS partitions (64 for head size 128: a context of 32768 tokens) cost one
-// memory round trip after the context length has arrived.
-constexpr uint32_t kMergeUnroll = 16; // partial rows in flight per thread
-
-template <int D>
+// UNROLL * ROWS partitions (64 for head size 128: a context of 32768 tokens) cost one
+// memory round trip after the context length has arrived.  Partial rows are fp16, or fp32 (T) over an int8 cache on
+// request: 16-byte loads, half as many in flight in the same registers.
+template <int D, typename T>
 struct MergeShape {
-  static constexpr uint32_t LANES_PER_ROW = D / 4;        // each lane owns 4 dims (8 bytes)
+  static constexpr uint32_t LANES_PER_ROW = D / 4;        // each lane owns 4 dims (8 or 16 bytes)
   static constexpr uint32_t ROWS = 128 / LANES_PER_ROW;   // partitions handled in parallel: 4 or 8
+  static constexpr uint32_t UNROLL = sizeof(T) == 4 ? 8u : 16u; // partial rows in flight per thread
 };
 
-template <int D>
+// N neighbouring elements of a partial row, as loaded
+template <typename T, uint32_t N>
+struct RowPiece;
+template <>
+struct RowPiece<__half, 4> {
+  uint2 raw;
+  __device__ __forceinline__ void clear() { raw = make_uint2(0u, 0u); }
+  __device__ __forceinline__ void load(const __half *p) { raw = __ldg(reinterpret_cast<const uint2 *>(p)); }
+  __device__ __forceinline__ void values(float (&x)[4]) const {
+    const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&raw.x));
+    const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&raw.y));
+    x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+  }
+};
+template <>
+struct RowPiece<__half, 2> {
+  uint32_t raw;
+  __device__ __forceinline__ void clear() { raw = 0u; }
+  __device__ __forceinline__ void load(const __half *p) { raw = __ldg(reinterpret_cast<const uint32_t *>(p)); }
+  __device__ __forceinline__ void values(float (&x)[2]) const {
+    const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&raw));
+    x[0] = a.x, x[1] = a.y;
+  }
+};
+template <>
+struct RowPiece<float, 4> {
+  float4 raw;
+  __device__ __forceinline__ void clear() { raw = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void load(const float *p) { raw = __ldg(reinterpret_cast<const float4 *>(p)); }
+  __device__ __forceinline__ void values(float (&x)[4]) const { x[0] = raw.x, x[1] = raw.y, x[2] = raw.z, x[3] = raw.w; }
+};
+template <>
+struct RowPiece<float, 2> {
+  float2 raw;
+  __device__ __forceinline__ void clear() { raw = make_float2(0.f, 0.f); }
+  __device__ __forceinline__ void load(const float *p) { raw = __ldg(reinterpret_cast<const float2 *>(p)); }
+  __device__ __forceinline__ void values(float (&x)[2]) const { x[0] = raw.x, x[1] = raw.y; }
+};
+
+template <int D, typename T>
 __global__ void __launch_bounds__(128, 8) // 64 registers: 1 184 CTAs resident, config 4's 1 024 pairs in one wave
-merge_partitions_kernel(__half *__restrict__ out, const __half *__restrict__ tmp_out,
+merge_partitions_kernel(__half *__restrict__ out, const T *__restrict__ tmp_out,
                         const float *__restrict__ max_logits, const float *__restrict__ exp_sums,
                         const uint32_t *__restrict__ context_lens, const uint32_t *__restrict__ seq_indices,
                         uint32_t num_heads, uint32_t max_num_partitions, uint32_t partition_size,
                         uint32_t ctx_limit, const uint32_t *__restrict__ table_offsets, uint32_t block_shift) {
-  constexpr uint32_t LANES_PER_ROW = MergeShape<D>::LANES_PER_ROW;
-  constexpr uint32_t ROWS = MergeShape<D>::ROWS;
-  constexpr uint32_t UNROLL = kMergeUnroll;
+  constexpr uint32_t LANES_PER_ROW = MergeShape<D, T>::LANES_PER_ROW;
+  constexpr uint32_t ROWS = MergeShape<D, T>::ROWS;
+  constexpr uint32_t UNROLL = MergeShape<D, T>::UNROLL;
   constexpr uint32_t WEIGHT_CACHE = 1024;           // weights kept in shared memory
   const uint32_t head = blockIdx.x;
   const uint32_t seq = (seq_indices != nullptr) ? __ldg(seq_indices + blockIdx.y) : blockIdx.y;
@@ -1742,12 +1792,12 @@ merge_partitions_kernel(__half *__restrict__ out, const __half *__restrict__ tmp
   // together with the context length, for every partition the scratch has room for: rows past
   // the context hold whatever the caller left there and are masked once the length is known.
   // One memory round trip instead of two.
-  uint2 raw[UNROLL];
+  RowPiece<T, 4> raw[UNROLL];
 #pragma unroll
   for (uint32_t u = 0; u < UNROLL; ++u) {
     const uint32_t p = row + u * ROWS;
-    raw[u] = (p < max_num_partitions) ? __ldg(reinterpret_cast<const uint2 *>(tmp_out + (base + p) * D + col))
-                                      : make_uint2(0u, 0u);
+    raw[u].clear();
+    if (p < max_num_partitions) raw[u].load(tmp_out + (base + p) * D + col);
   }
   float ml_own = (tid < max_num_partitions) ? max_logits[base + tid] : neg_infinity();
   float es_own = (tid < max_num_partitions) ? exp_sums[base + tid] : 0.f;
@@ -1791,13 +1841,13 @@ merge_partitions_kernel(__half *__restrict__ out, const __half *__restrict__ tmp
   };
 
   float a0 = 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
-  auto accumulate = [&](uint2 v, float w) {
-    const float2 v01 = __half22float2(*reinterpret_cast<const __half2 *>(&v.x));
-    const float2 v23 = __half22float2(*reinterpret_cast<const __half2 *>(&v.y));
-    a0 += w * v01.x;
-    a1 += w * v01.y;
-    a2 += w * v23.x;
-    a3 += w * v23.y;
+  auto accumulate = [&](const RowPiece<T, 4> &v, float w) {
+    float x[4];
+    v.values(x);
+    a0 += w * x[0];
+    a1 += w * x[1];
+    a2 += w * x[2];
+    a3 += w * x[3];
   };
   // partitions are taken in increasing order per thread: the sum has a fixed order
 #pragma unroll
@@ -1809,7 +1859,8 @@ merge_partitions_kernel(__half *__restrict__ out, const __half *__restrict__ tmp
 #pragma unroll
     for (uint32_t u = 0; u < UNROLL; ++u) {
       const uint32_t p = p0 + u * ROWS;
-      raw[u] = (p < np) ? __ldg(reinterpret_cast<const uint2 *>(tmp_out + (base + p) * D + col)) : make_uint2(0u, 0u);
+      raw[u].clear();
+      if (p < np) raw[u].load(tmp_out + (base + p) * D + col);
     }
 #pragma unroll
     for (uint32_t u = 0; u < UNROLL; ++u) {
@@ -1840,9 +1891,9 @@ merge_partitions_kernel(__half *__restrict__ out, const __half *__restrict__ tmp
 // (weights: four 32-wide shuffle trees added left to right; rows: one accumulator per
 // residue class p mod ROWS, classes added in increasing order), so both kernels produce the
 // same bits and the launcher may pick either.
-template <int D>
+template <int D, typename T>
 __global__ void __launch_bounds__(128)
-merge_partitions_warp_kernel(__half *__restrict__ out, const __half *__restrict__ tmp_out,
+merge_partitions_warp_kernel(__half *__restrict__ out, const T *__restrict__ tmp_out,
                              const float *__restrict__ max_logits, const float *__restrict__ exp_sums,
                              const uint32_t *__restrict__ context_lens,
                              const uint32_t *__restrict__ seq_indices, uint32_t num_heads,
@@ -1850,7 +1901,7 @@ merge_partitions_warp_kernel(__half *__restrict__ out, const __half *__restrict_
                              uint32_t ctx_limit, const uint32_t *__restrict__ table_offsets,
                              uint32_t block_shift) {
   constexpr uint32_t DPL = D / 32;                 // dims per lane: 4 or 2
-  constexpr uint32_t ROWS = MergeShape<D>::ROWS;   // residue classes of the CTA-per-pair kernel
+  constexpr uint32_t ROWS = MergeShape<D, T>::ROWS; // residue classes of the CTA-per-pair kernel
   const uint32_t lane = threadIdx.x & 31u;
   const uint32_t work = blockIdx.x * 4 + (threadIdx.x >> 5); // (position in the launch) * num_heads + head
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -1862,7 +1913,7 @@ merge_partitions_warp_kernel(__half *__restrict__ out, const __half *__restrict_
   const uint32_t ctx = merge_context(context_lens, seq, ctx_limit, table_offsets, block_shift);
   const uint32_t np = min(num_partitions_of(ctx, partition_size), max_num_partitions);
   const size_t base = static_cast<size_t>(pair) * max_num_partitions;
-  const __half *rows = tmp_out + base * D + lane * DPL;
+  const T *rows = tmp_out + base * D + lane * DPL;
 
   // the first 32 partitions' statistics live in registers, one partition per lane; their
   // rows are requested right away, before the weights are known
@@ -1870,14 +1921,11 @@ merge_partitions_warp_kernel(__half *__restrict__ out, const __half *__restrict_
   const float ml_lane = mine ? __ldg(max_logits + base + lane) : neg_infinity();
   const float es_lane = mine ? __ldg(exp_sums + base + lane) : 0.f;
   constexpr uint32_t PREFETCH = 2 * ROWS;
-  uint2 pre[PREFETCH];
+  RowPiece<T, DPL> pre[PREFETCH];
 #pragma unroll
   for (uint32_t u = 0; u < PREFETCH; ++u) {
-    pre[u] = make_uint2(0u, 0u);
-    if (u < np) {
-      if constexpr (DPL == 4) pre[u] = __ldg(reinterpret_cast<const uint2 *>(rows + static_cast<size_t>(u) * D));
-      else pre[u].x = __ldg(reinterpret_cast<const uint32_t *>(rows + static_cast<size_t>(u) * D));
-    }
+    pre[u].clear();
+    if (u < np) pre[u].load(rows + static_cast<size_t>(u) * D);
   }
   float m = ml_lane;
   for (uint32_t p = lane + 32; p < np; p += 32) m = fmaxf(m, max_logits[base + p]);
@@ -1902,15 +1950,11 @@ merge_partitions_warp_kernel(__half *__restrict__ out, const __half *__restrict_
   for (uint32_t r = 0; r < ROWS; ++r)
 #pragma unroll
     for (uint32_t i = 0; i < DPL; ++i) acc[r][i] = 0.f;
-  auto add_row = [&](uint32_t r, uint2 raw, float w) {
-    const float2 v01 = __half22float2(*reinterpret_cast<const __half2 *>(&raw.x));
-    acc[r][0] += w * v01.x;
-    acc[r][1] += w * v01.y;
-    if constexpr (DPL == 4) {
-      const float2 v23 = __half22float2(*reinterpret_cast<const __half2 *>(&raw.y));
-      acc[r][2] += w * v23.x;
-      acc[r][3] += w * v23.y;
-    }
+  auto add_row = [&](uint32_t r, const RowPiece<T, DPL> &piece, float w) {
+    float x[DPL];
+    piece.values(x);
+#pragma unroll
+    for (uint32_t i = 0; i < DPL; ++i) acc[r][i] += w * x[i];
   };
   // partitions 0 .. PREFETCH-1 from the prefetched rows (weights come from the owning lane)
 #pragma unroll
@@ -1926,12 +1970,11 @@ merge_partitions_warp_kernel(__half *__restrict__ out, const __half *__restrict_
 #pragma unroll
     for (uint32_t u = 0; u < PREFETCH; ++u) {
       const uint32_t p = p0 + u;
-      pre[u] = make_uint2(0u, 0u);
+      pre[u].clear();
       ml[u] = neg_infinity();
       es[u] = 0.f;
       if (p < np) {
-        if constexpr (DPL == 4) pre[u] = __ldg(reinterpret_cast<const uint2 *>(rows + static_cast<size_t>(p) * D));
-        else pre[u].x = __ldg(reinterpret_cast<const uint32_t *>(rows + static_cast<size_t>(p) * D));
+        pre[u].load(rows + static_cast<size_t>(p) * D);
         ml[u] = max_logits[base + p];
         es[u] = exp_sums[base + p];
       }

@@ -144,8 +144,12 @@ def check_scratch(p: _cabi.PaParams, max_logits, exp_sums, tem_output) -> None:
     s, h, npart, d = p.num_seqs, p.num_heads, p.max_num_partitions, p.head_size
     _require(tuple(max_logits.shape) == (s, h, npart) and tuple(exp_sums.shape) == (s, h, npart),
              "max_logits / exp_sums must be [num_seqs, num_heads, max_num_partitions]")
-    _require(tem_output.dtype == torch.float16 and tem_output.numel() >= s * h * npart * d,
-             "tem_output must be float16 [num_seqs, num_heads, max_num_partitions, head_size]")
+    if p.kv_dtype == _cabi.KV_INT8 and tem_output.dtype == torch.float32:
+        p.tmp_out_f32 = 1  # the split int8 operator keeps its partial rows in the scratch's type
+    else:
+        _require(tem_output.dtype == torch.float16, "tem_output must be float16 (int8 caches: or float32)")
+    _require(tem_output.numel() >= s * h * npart * d,
+             "tem_output must be [num_seqs, num_heads, max_num_partitions, head_size]")
 
 
 def run_entry(entry: str, p: _cabi.PaParams, device: torch.device) -> list[float]:

@@ -4,6 +4,8 @@ No reference counterpart: the surface is that of ``paged_attention_fp8_reduce`` 
 arguments, ``int8_scale`` in the place of ``fp8_scale``) over ``torch.int8`` caches, whose codes
 stand for code * scale.  The scale is ``int8_scale``, or one per KV head, or one for each block
 of tokens and KV head; ``cache_ops.append_block_scaled`` fills and keeps the latter.
+``tem_output`` may be float32 instead of float16: partial rows are then not rounded on their way
+to the merge (an error of 2.1e-4 of a result on average, its own rounding, instead of 2.9e-4).
 """
 from __future__ import annotations
 

@@ -42,7 +42,9 @@ class AutoDecodePlan:
 
     def __init__(self, context_lens_host: Sequence[int], num_heads: int, head_size: int, block_size: int,
                  max_blocks_per_seq: int, device, split_threshold_partitions: int = 2,
-                 fold_short_fraction: float = 0.25):
+                 fold_short_fraction: float = 0.25, partial_dtype: torch.dtype = torch.float16):
+        """`partial_dtype`: float32 keeps the partial rows of the split variant over an int8 cache unrounded
+        (`paged_attention_int8_reduce`); the other caches' take float16."""
         self.device = torch.device(device)
         self.psize = _cabi.partition_size(head_size)
         lens = [int(c) for c in context_lens_host]
@@ -57,7 +59,7 @@ class AutoDecodePlan:
         npart = max(1, (self.reduce.max_ctx + self.psize - 1) // self.psize) if self.reduce else 1
         self.max_logits = torch.empty(s, num_heads, npart, dtype=torch.float32, device=self.device)
         self.exp_sums = torch.empty_like(self.max_logits)
-        self.tmp_out = torch.empty(s, num_heads, npart, head_size, dtype=torch.float16, device=self.device)
+        self.tmp_out = torch.empty(s, num_heads, npart, head_size, dtype=partial_dtype, device=self.device)
         self.alibi = torch.ones(num_heads, dtype=torch.float32, device=self.device)
         self.streams = (torch.cuda.Stream(self.device), torch.cuda.Stream(self.device))
 

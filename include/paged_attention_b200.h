@@ -27,7 +27,8 @@
  *   out          fp16  [num_seqs, num_heads, head_size]
  *   max_logits   fp32  [num_seqs, num_heads, max_num_partitions]       (reduce only)
  *   exp_sums     fp32  [num_seqs, num_heads, max_num_partitions]       (reduce only)
- *   tmp_out      fp16  [num_seqs, num_heads, max_num_partitions, head_size] (reduce only)
+ *   tmp_out      fp16  [num_seqs, num_heads, max_num_partitions, head_size] (reduce only; fp32 of
+ *                the same extents with tmp_out_f32, int8 caches)
  *   sinks        fp16  [num_heads] or NULL
  */
 #ifndef PAGED_ATTENTION_B200_H_
@@ -91,7 +92,8 @@ typedef struct pa_params {
   float sm_scale;
   float fp8_scale; /* per-tensor dequantisation scale of an FP8 or int8 cache; ignored for fp16 */
   int32_t kv_dtype; /* pa_kv_dtype; must match the entry point (fp16, FP8 or int8) */
-  int32_t reserved1;
+  int32_t tmp_out_f32; /* launch_kernels_int8_reduce: non-zero if tmp_out holds fp32 elements, and partial
+                          rows are not rounded to fp16 on their way to the merge; ignored elsewhere */
   /* Optional per-KV-head dequantisation scales of an FP8 cache (device pointers, fp32
    * [num_kv_heads] each, or NULL).  The reference has one scalar fp8_scale
    * (paged_attention_fp8_loop/paged_attention_fp8_loop.cpp:34); when these are set,
