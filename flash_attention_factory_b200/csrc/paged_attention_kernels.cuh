@@ -1050,15 +1050,15 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
       }
     };
     // Running reference of the V block scales: a tile's weights are multiplied by its
-    // scale over the largest scale so far, a factor of at most 1, before they are rounded to fp16,
+    // scale over the largest scale so far, a factor of at most 1 in size, before they are rounded to fp16,
     // and the accumulator carries the reference; multiplying by the scale itself would push the
     // weights of a cache with small values into the subnormal halves (a block scale of e5m2 is its largest value
     // over 57344: 1.7e-5 for values of 1, below every normal half already).  Uniform across the warp;
     // the reference grows about ln(blocks) times per item.
     float v_ref = 0.f, v_inv = 0.f;
     auto fold_v_scales = [&](const float (&va)[VH], const float (&vb)[VH], float (&wa)[VH], float (&wb)[VH]) {
-      float top = fmaxf(va[0], vb[0]);
-      if constexpr (VH == 2) top = fmaxf(top, fmaxf(va[1], vb[1]));
+      float top = fmaxf(fabsf(va[0]), fabsf(vb[0])); // FP8 block scales may be negative
+      if constexpr (VH == 2) top = fmaxf(top, fmaxf(fabsf(va[1]), fabsf(vb[1])));
       if (top > v_ref) {
         const float next = fmaxf(top, 0x1p-126f); // the reciprocal of a subnormal scale would be infinite
         const float r = v_ref / next;

@@ -34,6 +34,29 @@ def test_wide_launch_gives_the_bits_of_the_narrow_one(cuda_device):
 
 @pytest.mark.parametrize("variant", ["loop", "reduce"])
 @pytest.mark.parametrize("cache", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("hk,d,bs", [(4, 128, 16), (2, 64, 64), (8, 64, 16)])
+def test_negative_scales(cuda_device, variant, cache, hk, d, bs):
+    """A block's FP8 scales are factors of any sign: V negative throughout, or in some blocks; K in some."""
+    case = paged_case(90 + hk, [1, 700, 2049, 33], 2 * hk, hk, d, bs, cache=cache, spread=4.0)
+    sizes = {n: case[f"{n}_scale"] for n in "kv"}
+    sign = 1.0 - 2.0 * (torch.rand(sizes["v"].shape, generator=torch.Generator().manual_seed(4)) < 0.5)
+    for k_sign, v_sign in ((1.0, -1.0), (1.0, sign), (sign.flip(0), sign)):
+        case["k_scale"], case["v_scale"] = sizes["k"] * k_sign, sizes["v"] * v_sign
+        got = attend("fp8", variant, case, cuda_device, k_scale_per_block=case["k_scale"], v_scale_per_block=case["v_scale"])
+        check(got, *attention64(case, case["k_scale"], case["v_scale"]), f"{cache} {variant}")
+
+
+@pytest.mark.parametrize("hk,group", [(4, 2), (1, 3)])
+def test_many_short_sequences(cuda_device, hk, group):
+    """Whole-context items of the persistent form, with a warp per head and with warps that share one."""
+    lens = torch.randint(0, 90, (700,), generator=torch.Generator().manual_seed(1)).tolist()
+    case = paged_case(95, lens, hk * group, hk, 64, 16, cache="e5m2", spread=6.0)
+    got = attend("fp8", "loop", case, cuda_device, k_scale_per_block=case["k_scale"], v_scale_per_block=case["v_scale"])
+    check(got, *attention64(case, case["k_scale"], case["v_scale"]), f"hk{hk}")
+
+
+@pytest.mark.parametrize("variant", ["loop", "reduce"])
+@pytest.mark.parametrize("cache", ["e4m3", "e5m2"])
 def test_what_the_append_stored_is_read_back(cuda_device, variant, cache):
     """append_block_scaled over prompts with values of about 0.1, then attention over the caches and scales it left."""
     from flash_attention_factory_b200.cache_ops import append_block_scaled
