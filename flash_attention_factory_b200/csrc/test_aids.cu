@@ -214,6 +214,7 @@ PA_API int pa_aid_diff_split(const pa_params *p, uint32_t *partition_tokens, uin
   if (p == nullptr || partition_tokens == nullptr || box_rows == nullptr)
     return fail(PA_ERR_BAD_ARG, "diff_split: null argument");
   if (int rc = validate_params(p, p->kv_dtype != PA_KV_F16, /*needs_scratch=*/true, p->kv_dtype == PA_KV_INT8)) return rc;
+  if (p->num_seqs == 0) return fail(PA_ERR_BAD_ARG, "diff_split: no sequences");
   *partition_tokens = diff_partition_tokens(p);
   *box_rows = diff_box_rows(p);
   return PA_OK;
