@@ -234,7 +234,7 @@ constexpr uint32_t kStageBytes = PASSES * 2 * 32 * 16; // one job's rows of a wa
 // maxima propagate NaNs, so an infinity or a NaN among the inputs shows in the result.  A lane without a row of its
 // own in a group takes the last row over again: it changes no maximum and is not stored.
 // Measured on 37 364 prompt tokens (8 KV heads of 128, e4m3, rotated): rows in registers, read when their job comes,
-// 79 us; with the copies ahead, pairs of values per instruction and whole runs of addresses per piece 74 us (51 us
+// 79 us; with the copies ahead, pairs of values per instruction and whole runs of addresses per piece 72 us (51 us
 // without the rotation, whose angles come from the L1 cache twice for every head; 38 us is what the bytes take).
 // Layout: [row group][piece][lane], 16 bytes each.
 template <int PASSES, bool ROTATE, bool INTERLEAVED>
@@ -596,7 +596,9 @@ extern "C" PA_API int pa_append_block_scaled(const pa_block_scaled_params *p, vo
   while (per_cta < 32u && per_cta * 2u <= average) per_cta *= 2u;
   a.tokens_per_cta = per_cta;
   // A few new rows per block (decode steps): one group of rows per warp, and twice the CTAs on an SM.  Otherwise four
-  // groups, and as many warps to a job as hold a block's new rows in shared memory.
+  // groups, and as many warps to a job as hold a block's new rows in shared memory.  (By the average: where many decode
+  // tokens come with a prompt chunk, the chunk's rows take the general way, right but slow: 255 tokens and a chunk
+  // of 2048, int8, 8 KV heads of 128, 24 us instead of the 9 that the chunk takes alone.)
   const uint32_t rows = std::min(p->block_size, average);
   const uint32_t rows_per_pass = 32u / (p->head_size / 16u);
   const bool few = rows <= rows_per_pass;

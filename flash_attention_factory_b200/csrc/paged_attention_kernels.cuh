@@ -584,7 +584,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
   //   differential, fp16, 48 sequences up to 8192 tokens   3.2e-4 -> 2.1e-4   135 -> 138 us
   //   differential, e4m3, 2 x 65536 tokens                 3.2e-4 -> 2.1e-4    59 ->  70 us
   //   int8 loop, 64 x 1500 tokens, head size 64            2.8e-4 -> 2.1e-4    28 -> 29.5 us
-  //   int8 split, 128 sequences up to 8192 tokens          3.5e-4 -> 2.9e-4   152 -> 155 us (fp16 partial rows)
+  //   int8 split, 128 sequences up to 8192 tokens          3.5e-4 -> 2.9e-4   152 -> 155 us (fp16 partial rows; fp32
+  //                                                                  2.1e-4, same time)
   // The second case shows what it costs where the MMAs' fixed latencies are the bound (two warps to a scheduler):
   // other orders of the MMAs, V fragments fetched ahead and weights packed later (with a third of the spills) changed
   // nothing.  Ordinary attention over fp16 and FP8 caches takes one part.
@@ -794,8 +795,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k,
         const uint32_t stages_in_batch = divide_round_up(chunks_in_batch, chunks_per_stage);
         for (uint32_t sb = 0; sb < stages_in_batch; ++sb) {
           // Every lane waits, because every lane may copy into the stage: what the consumers have read of it is ordered
-          // before a lane's own copies by that lane's own wait (a wait of lane 0 and a shuffle order no memory).  No
-          // slower: 64 x 4096 tokens of e5m2, head size 64, 75 -> 70 us; 128 x 8192 of e4m3 330 -> 327.
+          // before a lane's own copies by that lane's own wait (a wait of lane 0 and a shuffle order no memory).
+          // Measured against that: 1024 log-normal contexts of e5m2 989 -> 972 us; 64 x 4096 tokens of e5m2, head size
+          // 64, 75 -> 70; 64 x 1500 tokens of fp16, head size 64, loop, 36.1 -> 36.5.
           alive = mbar_wait_bounded(&empty_bar[slot], phase ^ 1u, abort_flag);
           alive = __all_sync(0xffffffffu, alive ? 1 : 0) != 0;
           if (!alive) break;

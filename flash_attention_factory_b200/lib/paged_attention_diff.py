@@ -31,7 +31,8 @@ def _kv_dtype(cache: torch.Tensor) -> int:
 
 def scratch(query: torch.Tensor, key_cache: torch.Tensor, max_context_len: int):
     """(max_logits, exp_sums, tem_output) for calls of this shape: float32 [S, 2 H, NP], the same, and
-    [S, 2 H, NP, 2 D].  NP sets how finely a context is split; any NP >= 1 gives a correct result."""
+    [S, 2 H, NP, 2 D].  NP sets how finely a context is split; any NP >= 1 gives a correct result.  For large batches
+    of long contexts that is memory: 256 sequences of 32768 tokens with 32 heads of 128 over an fp16 cache get 2.1 GB."""
     s, h2, d = query.shape
     kv_dtype = _kv_dtype(key_cache)
     hint = max(0, min(int(max_context_len), 0xFFFFFFFF))
